@@ -124,7 +124,7 @@ def _quantize(rows):
     fine = torch.isfinite(x)
     a = torch.where(fine, x.abs(), 0).amax(-1)
     m, e = torch.frexp(a)                                                                # a = m 2^e, 1/2 <= m < 1
-    e = torch.where(a == 0, 0, (e - 9 + (m > 0.875)).clamp(min=-127))
+    e = torch.where(a == 0, 0, (e - 9 + (m > 0.875)).clamp(min=-100))
     half = -(e // 2)                                                                     # 2^-e in two factors that are both ordinary floats
     c = x * torch.exp2(half.float()).unsqueeze(-1) * torch.exp2((-e - half).float()).unsqueeze(-1)
     codes = torch.where(fine, c, float("nan")).to(torch.float8_e4m3fn)
