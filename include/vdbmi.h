@@ -134,6 +134,74 @@ vdb_status vdb_score_scan(const float* queries, size_t nq, const float* base, si
 vdb_status vdb_score_scan_dev(const float* d_queries, size_t nq, const float* d_base, size_t n, size_t dim, size_t stride,
                               vdb_metric metric, vdb_arith arith, float* d_out, void* stream);
 
+/* ---------------------------------------------------------------- 8-bit rows ---------------
+ * Extension (the reference keeps f32 rows only, types.rs:9).  A row is cut into blocks of 128 columns; a block is held as
+ * 8-bit floating-point codes (e4m3: sign, 4 exponent bits, 3 fraction bits, largest value 448, no infinities, 0x7F = NaN) and
+ * one power-of-two scale.  value = code * 2^(scale - 127).  With a = the largest finite |x| of the block, the scale is the
+ * smallest power of two with a <= 448 * scale (at least 2^-100; 1 for a block of zeros), a code is x / scale rounded to
+ * nearest, ties to even, and at most 240 where the scale is 2^120 (so that every value is finite in f32); infinities and NaN
+ * become the NaN code.
+ *
+ * Everything below reads and writes device memory, enqueues on `stream` (NULL = the null stream) and returns without waiting;
+ * nothing is allocated, so the calls may be captured into a graph and may overlap on different streams.  The work runs on the
+ * device that owns the buffers, which must be one; the calling thread's current device is left as it was.  Host memory that
+ * the device cannot read, NULL pointers, impossible sizes and misaligned buffers are VDB_ERR_ARGUMENT and nothing is launched;
+ * zero rows or queries are VDB_OK and nothing is launched. */
+
+/* Element types of the rows handed to vdb_q8_quantize_dev. */
+typedef enum { VDB_F32 = 0, VDB_F16 = 1, VDB_BF16 = 2 } vdb_dtype;
+
+/* n rows of `dim` columns in device memory.
+ *   codes   n x code_stride bytes, 16-byte aligned, code_stride a multiple of 16 and >= dim; the bytes from dim to the next
+ *           multiple of 16 must be zero (the quantiser writes them), bytes beyond that are neither read nor written
+ *   scales  n x scale_stride bytes, 4-byte aligned, scale_stride a multiple of 4 and >= the number of blocks; the bytes from the
+ *           last block to the next multiple of 4 are written as 127 and their values do not matter.  27 .. 247 are scales, 255 makes
+ *           every score of its row NaN, others (values beyond f32, or too small for it) are not supported
+ *   norms2  n sums of the squared values (nullable: not written; needed by cosine and Euclidean scores)
+ * dim <= 2^24, n < 2^32.  The struct itself is read during the call only. */
+typedef struct {
+    uint8_t* codes; uint8_t* scales; float* norms2;
+    size_t n, dim, code_stride, scale_stride;
+} vdb_q8_rows;
+
+/* The smallest strides for rows of `dim` columns. */
+vdb_status vdb_q8_strides(size_t dim, size_t* code_stride, size_t* scale_stride);
+/* Fill `out` (its n, dim, strides and buffers are the caller's) from n rows that lie `stride` elements apart (>= dim).  Rows of
+ * any alignment that fits their element type; rows whose starts are all 16-byte (16-bit types: 8-byte) aligned are read fastest. */
+vdb_status vdb_q8_quantize_dev(const void* d_rows, vdb_dtype dtype, size_t stride, const vdb_q8_rows* out, void* stream);
+/* d_out[q * out_stride + i] = score of queries row q and base row i over the held values (score(), metric.rs:4-35): dot;
+ * 1 - dot / (|q||i| + 1e-10); sqrt(max(0, |q|^2 + |i|^2 - 2 dot)) - the last one loses the digits that |q|^2 + |i|^2 and
+ * 2 dot share.  Products are exact, sums are held in 32 bits.  out_stride >= base->n; d_out must not overlap the rows. */
+vdb_status vdb_q8_score_dev(const vdb_q8_rows* queries, const vdb_q8_rows* base, vdb_metric metric, float* d_out, size_t out_stride, void* stream);
+/* vdb_score_scan over 8-bit rows: host buffers in f32, quantised and scored on `device`, out[q * n + i]. */
+vdb_status vdb_q8_score_scan(const float* queries, size_t nq, const float* base, size_t n, size_t dim, vdb_metric metric, int device, float* out);
+
+/* ---------------------------------------------------------------- score rows ---------------
+ * Extension: what is laid over dense score rows (vdb_score_scan_dev, vdb_q8_score_dev, or any nq x n f32 table where a column is
+ * a row, a product, a token) before the best are taken.  Calls as described at the 8-bit rows.  With g = the score where higher is
+ * better (VDB_DOT) and g = -score for the distances (VDB_COSINE, VDB_EUCLIDEAN), for each query and column in this order:
+ *   seen c > 0 times:  g = g > 0 ? g / repeat : g * repeat;   g = g - (frequency * c + presence)
+ *   boost:             g = g + boost
+ *   not passing:       g = -infinity, whatever the score was (NaN too)
+ * and the result is g or -g.  Every member may be left out (NULL). */
+typedef struct {
+    const uint32_t* pass;         /* bit i of word w: column 32 w + i passes (the layout of vdb_segment_filter_bitmaps); (n + 31) / 32 words per row */
+    size_t pass_stride;           /* words from one query's bitmap to the next; 0 = one bitmap for all queries */
+    const float* boost;           /* n floats per row, added */
+    size_t boost_stride;          /* floats from one query's row to the next; 0 = one row for all queries */
+    const uint32_t* seen;         /* n_seen columns: query q has seen seen[seen_offsets[q]] .. seen[seen_offsets[q + 1] - 1]; a column that
+                                   * occurs c times counts c; entries >= n are passed over */
+    const uint64_t* seen_offsets; /* nq + 1, ascending, at most n_seen (larger ones are cut to n_seen) */
+    size_t n_seen;
+    const float* repeat;          /* per query, > 0; NULL = 1 */
+    const float* frequency;       /* per query; NULL = 0 */
+    const float* presence;        /* per query; NULL = 0 */
+} vdb_score_adjust;
+/* d_scores: nq rows of n floats, `stride` apart.  d_out (rows out_stride apart) may be d_scores itself with the same stride;
+ * any other overlap is VDB_ERR_ARGUMENT.  Floats of a row beyond n are left as they are. */
+vdb_status vdb_score_adjust_dev(const float* d_scores, size_t stride, size_t nq, size_t n, vdb_metric metric, const vdb_score_adjust* how,
+                                float* d_out, size_t out_stride, void* stream);
+
 /* ---------------------------------------------------------------- payload.rs -------------- */
 
 vdb_value* vdb_value_int(int64_t v);

@@ -111,6 +111,17 @@ class LayerCsrC(C.Structure):
                 ("n_edges", C.c_size_t)]
 
 
+class Q8RowsC(C.Structure):              # vdb_q8_rows
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("norms2", C.c_void_p),
+                ("n", C.c_size_t), ("dim", C.c_size_t), ("code_stride", C.c_size_t), ("scale_stride", C.c_size_t)]
+
+
+class ScoreAdjustC(C.Structure):         # vdb_score_adjust
+    _fields_ = [("pass_bits", C.c_void_p), ("pass_stride", C.c_size_t), ("boost", C.c_void_p), ("boost_stride", C.c_size_t),
+                ("seen", C.c_void_p), ("seen_offsets", C.c_void_p), ("n_seen", C.c_size_t),
+                ("repeat", C.c_void_p), ("frequency", C.c_void_p), ("presence", C.c_void_p)]
+
+
 class ScoredPoint:
     """ScoredPoint (hnsw.rs:11-23): equality compares sort_key only, as the reference's PartialEq."""
     __slots__ = ("id", "raw_score", "sort_key")
@@ -202,6 +213,11 @@ _SIGS = {
     "segment_insert_batch_columns": (_I, [_VP, _VP, _SZ, _SZ, _SZ, _VP, _VP, _VP, _VP]),
     "topk_merge_dev": (_I, [_VP, _VP, _SZ, _SZ, _SZ, _VP, _VP, _VP]),
     "score_scan_dev": (_I, [_VP, _SZ, _VP, _SZ, _SZ, _SZ, _I, _I, _VP, _VP]),
+    "q8_strides": (_I, [_SZ, _PSZ, _PSZ]),
+    "q8_quantize_dev": (_I, [_VP, _I, _SZ, _VP, _VP]),
+    "q8_score_dev": (_I, [_VP, _VP, _I, _VP, _SZ, _VP]),
+    "q8_score_scan": (_I, [_VP, _SZ, _VP, _SZ, _SZ, _I, _I, _VP]),
+    "score_adjust_dev": (_I, [_VP, _SZ, _SZ, _SZ, _I, _VP, _VP, _SZ, _VP]),
     "default_options": (None, [_VP]),
     "shard_group_unique_id": (_I, [_VP, _SZ]), "shard_group_new": (_I, [_VP, _SZ, _I, _I, _I, C.POINTER(_VP)]),
     "shard_group_free": (None, [_VP]), "shard_group_size": (_I, [_VP]), "shard_group_rank": (_I, [_VP]),
@@ -380,6 +396,15 @@ def bind(cdll, prefix="vdb_", required=None):
         q, b = _f32(queries), _f32(base)
         out = np.zeros((q.shape[0], b.shape[0]), dtype=np.float32)
         check(fn.score_scan(_ptr(q), q.shape[0], _ptr(b), b.shape[0], q.shape[1], int(metric), int(arith), device, _ptr(out)))
+        return out
+
+    def q8_score_scan(queries, base, metric, device=0):
+        """score_scan over rows held in 8 bits (vdb_q8_score_scan)."""
+        q, b = _f32(queries), _f32(base)
+        if q.ndim != 2 or b.ndim != 2: raise ArgumentError("queries and base are matrices of rows")
+        if q.shape[1] != b.shape[1]: raise VectorLengthMismatch(f"Vector length mismatch: expected {b.shape[1]}, got {q.shape[1]}")
+        out = np.zeros((q.shape[0], b.shape[0]), dtype=np.float32)
+        check(fn.q8_score_scan(_ptr(q), q.shape[0], _ptr(b), b.shape[0], q.shape[1], int(metric), device, _ptr(out)))
         return out
 
     class HNSWIndex:
@@ -604,6 +629,6 @@ def bind(cdll, prefix="vdb_", required=None):
         InvalidPayload=InvalidPayload, SearchError=SearchError, ReferencePanic=ReferencePanic,
         DeviceError=DeviceError, ArgumentError=ArgumentError,
         ScoredPoint=ScoredPoint, PayloadValue=PayloadValue, Payload=Payload, Filter=Filter,
-        evaluate_filter=evaluate_filter, PayloadIndex=PayloadIndex, score=score, score_scan=score_scan,
+        evaluate_filter=evaluate_filter, PayloadIndex=PayloadIndex, score=score, score_scan=score_scan, q8_score_scan=q8_score_scan,
         HNSWIndex=HNSWIndex, Segment=Segment, SCORED_DTYPE=SCORED_DTYPE, STATS_DTYPE=STATS_DTYPE,
     )

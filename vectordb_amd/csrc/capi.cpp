@@ -2,18 +2,12 @@
 #include <cstdio>
 #include <cstring>
 
+#include "guard.hpp"
 #include "index.hpp"
 
 using namespace vdb;
 
 namespace {
-template <class F> vdb_status guard(F&& f) {
-    try { f(); return VDB_OK; }
-    catch (const Failure& e) { set_last_error(e.e.msg); return e.e.code; }
-    catch (const std::bad_alloc&) { set_last_error("out of host memory"); return VDB_ERR_DEVICE; }
-    catch (const std::exception& e) { set_last_error(std::string("internal error: ") + e.what()); return VDB_ERR_PANIC; }
-}
-void need(const void* p, const char* what) { if (!p) throw Failure(err_arg(std::string(what) + " is NULL")); }
 void emit(const std::vector<vdb_scored_point>& v, vdb_scored_point* out, size_t* out_n) {
     if (!v.empty()) std::memcpy(out, v.data(), v.size() * sizeof(vdb_scored_point));
     if (out_n) *out_n = v.size();

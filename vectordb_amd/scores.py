@@ -1,0 +1,191 @@
+"""Dense scores on device tensors: rows held in 8 bits, their block-scaled product, and what is laid over score rows.
+
+    base = quantize_rows(vectors)                        # once: f32 / f16 / bf16 tensor [n, dim] -> Q8Rows
+    q = quantize_rows(queries)                           # per batch
+    s = score_rows(q, base, DistanceMetric.Cosine)       # [nq, n] f32
+    s = adjust_scores(s, DistanceMetric.Cosine, pass_bits=bits, boost=boost, seen=seen, seen_offsets=offsets, frequency=f)
+
+Each call is one entry point of the C ABI (vdb_q8_quantize_dev, vdb_q8_score_dev, vdb_score_adjust_dev: include/vdbmi.h has
+the formulas and the layout), enqueued on the current stream of the tensors' device; nothing waits.  Tensors must live on one
+GPU; what a call cannot take is refused with ArgumentError before anything is launched, or VectorLengthMismatch for rows of two lengths.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from .capi import ArgumentError, DistanceMetric, Q8RowsC, ScoreAdjustC, VectorLengthMismatch
+
+BLOCK = 128                               # columns that share one scale
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_METRICS = frozenset(int(m) for m in DistanceMetric)
+
+
+def _api():
+    from . import api
+    return api()
+
+
+def _stream(t):
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _refuse(why):
+    raise ArgumentError(why)
+
+
+def _check(t, what, dtype, ndim, device=None):
+    """A tensor of one type and rank whose last axis is dense; -> elements from row to row."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != ndim:
+        _refuse(f"{what}: expected a {ndim}-d {dtype} tensor")
+    if device is not None and t.device != device:
+        _refuse(f"{what} is on {t.device}, not on {device}")
+    if not t.numel():
+        return t.shape[-1]
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        _refuse(f"{what}: the last axis must be dense")
+    if ndim == 2 and t.shape[0] > 1:
+        if t.stride(0) < t.shape[1]:
+            _refuse(f"{what}: rows overlap")
+        return t.stride(0)
+    return t.shape[-1]
+
+
+def _on_gpu(t, what):
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+        _refuse(f"{what} must be a tensor on the GPU")
+
+
+def _metric(m):
+    if int(m) not in _METRICS:
+        _refuse("unknown metric")
+    return int(m)
+
+
+def _out(out, nq, n, device):
+    if out is None:
+        return torch.empty(nq, n, dtype=torch.float32, device=device), n
+    stride = _check(out, "out", torch.float32, 2, device)
+    if tuple(out.shape) != (nq, n):
+        _refuse(f"out: expected shape {(nq, n)}")
+    return out, stride
+
+
+class Q8Rows:
+    """Rows of `dim` columns as e4m3 codes (uint8 [n, >= dim, a multiple of 16]), one power-of-two scale per block of 128
+    columns (uint8 [n, >= blocks, a multiple of 4]: exponent + 127) and squared norms (f32 [n], or None: dot products only)."""
+    __slots__ = ("codes", "scales", "norms2", "dim", "_c")
+
+    def __init__(self, codes, scales, norms2, dim):
+        _on_gpu(codes, "codes")
+        cs, ss = _check(codes, "codes", torch.uint8, 2), _check(scales, "scales", torch.uint8, 2, codes.device)
+        n, dim = codes.shape[0], int(dim)
+        if dim < 1 or codes.shape[1] < -(-dim // 16) * 16 or scales.shape[1] < -(-dim // (4 * BLOCK)) * 4:
+            _refuse("codes or scales are narrower than a row")
+        if scales.shape[0] != n:
+            _refuse("codes and scales hold different numbers of rows")
+        if norms2 is not None:
+            _check(norms2, "norms2", torch.float32, 1, codes.device)
+            if norms2.shape[0] != n:
+                _refuse("codes and norms2 hold different numbers of rows")
+        self.codes, self.scales, self.norms2, self.dim = codes, scales, norms2, dim
+        self._c = Q8RowsC(codes.data_ptr(), scales.data_ptr(), norms2.data_ptr() if norms2 is not None else None, n, dim, cs, ss)
+
+    @classmethod
+    def empty(cls, n, dim, device):
+        """Room for n rows."""
+        if dim < 1 or n < 0:
+            _refuse("empty rows")
+        wide, blocks = -(-dim // 16) * 16, -(-dim // (4 * BLOCK)) * 4
+        return cls(torch.empty(n, wide, dtype=torch.uint8, device=device), torch.empty(n, blocks, dtype=torch.uint8, device=device),
+                   torch.empty(n, dtype=torch.float32, device=device), dim)
+
+    def __len__(self):
+        return self.codes.shape[0]
+
+    def __getitem__(self, rows):
+        """A range of rows, sharing memory."""
+        if not isinstance(rows, slice) or rows.step not in (None, 1):
+            _refuse("rows are taken by ranges")
+        return Q8Rows(self.codes[rows], self.scales[rows], None if self.norms2 is None else self.norms2[rows], self.dim)
+
+
+def quantize_rows(rows, out=None):
+    """f32 / f16 / bf16 rows [n, dim] -> Q8Rows (into `out` where given: appending is quantize_rows(new, out=room[n:n + k]))."""
+    _on_gpu(rows, "rows")
+    if rows.dtype not in _DTYPES:
+        _refuse("rows: expected f32, f16 or bf16")
+    stride = _check(rows, "rows", rows.dtype, 2)
+    n, dim = rows.shape
+    if out is None:
+        out = Q8Rows.empty(n, dim, rows.device)
+    elif len(out) != n or out.dim != dim or out.codes.device != rows.device:
+        _refuse(f"out: expected {n} rows of {dim} columns on {rows.device}")
+    api = _api()
+    api.check(api.fn.q8_quantize_dev(rows.data_ptr(), _DTYPES[rows.dtype], stride, C.byref(out._c), _stream(rows)))
+    return out
+
+
+def score_rows(queries, base, metric, out=None):
+    """Scores [nq, n] of every query (Q8Rows) against every row (Q8Rows)."""
+    if not isinstance(queries, Q8Rows) or not isinstance(base, Q8Rows):
+        _refuse("queries and base are Q8Rows")
+    dev = base.codes.device
+    if queries.codes.device != dev:
+        _refuse(f"queries are on {queries.codes.device}, not on {dev}")
+    if queries.dim != base.dim:
+        raise VectorLengthMismatch(f"Vector length mismatch: expected {base.dim}, got {queries.dim}")
+    out, stride = _out(out, len(queries), len(base), dev)
+    api = _api()
+    api.check(api.fn.q8_score_dev(C.byref(queries._c), C.byref(base._c), _metric(metric), out.data_ptr(), stride, _stream(out)))
+    return out
+
+
+def adjust_scores(scores, metric, *, pass_bits=None, boost=None, seen=None, seen_offsets=None, repeat=None, frequency=None, presence=None, out=None):
+    """What vdb_score_adjust describes, over scores [nq, n] f32 (a tensor of its own, or `out`; out=scores works in place).
+
+    pass_bits: int32 [words] or [1 or nq, words], words = ceil(n / 32); boost: f32 [n] or [1 or nq, n]; seen: int32 columns of all
+    queries behind each other (read as unsigned; those >= n are passed over), seen_offsets: int64 [nq + 1]; repeat / frequency / presence: f32 [nq]."""
+    _on_gpu(scores, "scores")
+    dev = scores.device
+    stride = _check(scores, "scores", torch.float32, 2)
+    nq, n = scores.shape
+    metric = _metric(metric)
+    how = ScoreAdjustC()
+
+    def per_query(t, what, dtype, width):
+        if t.dim() == 1:
+            t = t.unsqueeze(0)
+        s = _check(t, what, dtype, 2, dev)
+        if t.shape[1] < width or t.shape[0] not in (1, nq):
+            _refuse(f"{what}: expected 1 or {nq} rows of {width}")
+        return t.data_ptr(), s if t.shape[0] > 1 else 0
+
+    if pass_bits is not None:
+        how.pass_bits, how.pass_stride = per_query(pass_bits, "pass_bits", torch.int32, -(-n // 32))
+    if boost is not None:
+        how.boost, how.boost_stride = per_query(boost, "boost", torch.float32, n)
+    if (seen is None) != (seen_offsets is None):
+        _refuse("seen and seen_offsets come together")
+    if seen is not None:
+        _check(seen, "seen", torch.int32, 1, dev)
+        _check(seen_offsets, "seen_offsets", torch.int64, 1, dev)
+        if seen_offsets.shape[0] != nq + 1:
+            _refuse(f"seen_offsets: expected {nq + 1}")
+        how.n_seen = seen.shape[0]
+        if how.n_seen:
+            how.seen, how.seen_offsets = seen.data_ptr(), seen_offsets.data_ptr()
+    for what, t in (("repeat", repeat), ("frequency", frequency), ("presence", presence)):
+        if t is None:
+            continue
+        _check(t, what, torch.float32, 1, dev)
+        if seen is None:
+            _refuse(f"{what} without seen")
+        if t.shape[0] != nq:
+            _refuse(f"{what}: expected {nq}")
+        setattr(how, what, t.data_ptr())
+    out, out_stride = _out(out, nq, n, dev)
+    api = _api()
+    api.check(api.fn.score_adjust_dev(scores.data_ptr(), stride, nq, n, metric, C.byref(how), out.data_ptr(), out_stride, _stream(scores)))
+    return out
