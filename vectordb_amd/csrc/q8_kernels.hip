@@ -3,6 +3,7 @@
 #include <hip/hip_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "q8.hpp"
 
@@ -10,6 +11,7 @@ namespace vdb {
 namespace {
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 // ---------------------------------------------------------------- quantiser
 // Block of 128 columns, a = max |x| over its finite values: e = the smallest exponent from -100 on with a <= 448 * 2^e, code =
@@ -35,6 +37,7 @@ template <class T, bool VEC> __device__ inline void load_four(const T* row, uint
     }
 }
 
+constexpr size_t MAX_STRIDE = 1u << 24;     // of the rows that the tiled kernel takes: its offsets have 32 bits
 constexpr int MIN_EXP = -100, TOP_EXP = 120;
 
 template <class T, bool VEC>
@@ -111,11 +114,263 @@ __device__ inline bf16x8 widen(uint32_t lo, uint32_t hi, float scale) {         
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// Roots and reciprocals are the hardware's (one step off at most): the scores are FAST arithmetic.
+__device__ inline float root(float x) { return __builtin_amdgcn_sqrtf(x); }
+// What a row's (query's) squared norm is used as.
+__device__ inline float norm_of(const float* norms2, size_t i, int metric) {
+    return metric == VDB_DOT ? 0.f : metric == VDB_COSINE ? root(norms2[i]) : norms2[i];
+}
 __device__ inline float finish(float dot, float nq, float nb, int metric) {
     if (metric == VDB_DOT) return dot;
-    if (metric == VDB_COSINE) return 1.0f - dot / (__builtin_sqrtf(nq) * __builtin_sqrtf(nb) + 1e-10f);
+    if (metric == VDB_COSINE) return __builtin_fmaf(-dot, __builtin_amdgcn_rcpf(__builtin_fmaf(nq, nb, 1e-10f)), 1.0f);
     const float d = __builtin_fmaf(-2.f, dot, nq + nb);
-    return __builtin_sqrtf(d < 0.f ? 0.f : d);                 // NaN stays
+    return root(d < 0.f ? 0.f : d);                            // NaN stays
+}
+
+// Many queries: a workgroup scores BM rows against BN queries at a time, a wavefront WM x WN of them in 32 x 32 tiles; the grid is
+// what the chip holds and every workgroup walks through its tiles.  Both sides' codes go through a ring of S buffers in LDS, 64
+// columns a step.  While a step is multiplied, the next one has arrived and the S - 2 behind it are on their way (straight to LDS, 16
+// bytes per lane), those of the next tile too, so that a tile's first step waits for nothing; one barrier per step hands a buffer on,
+// and the first fragments of a step are read before it.  A row's 16-byte chunk c lies at place c ^ (row / 4 mod 4): the eight rows
+// that an LDS read serves at a time fall on different banks.
+// v_mfma_f32_32x32x16_bf16: lane (r, g) holds eight columns of query (row) r; one 16-byte chunk makes two such operands (chunk
+// 2 h + g in half h of the step).  Codes are widened when they are read: per 32 columns 8 conversions for each of the WM / 32 + WN / 32
+// fragments, and WM WN / 512 matrix instructions of eight times their length.  The queries are the left operand: a result register
+// holds 32 rows of two queries.  Slot 32 i + r of WM holds row MT r + i (MT = WM / 32), so that MT registers of a lane are consecutive
+// rows: a store writes 128 MT bytes in a row for each of two queries.
+// The scales of four blocks are one word per row, which comes with every step.
+__device__ const uint4 zero16[1] = {};
+
+// A wavefront's load straight to LDS: lane i's BYTES bytes at base + off (p) go to dst + i * BYTES.  Written as assembly because the
+// compiler makes every LDS read behind such a load wait for it, whatever buffer it goes to; step_barrier() waits for the right ones.
+// The instructions write no register.
+__device__ inline void load16_to_lds(const uint8_t* base, uint32_t off, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(dst) : "memory");
+}
+__device__ inline void load16_to_lds(const void* p, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(p), "s"(dst) : "memory");
+}
+__device__ inline void load4_to_lds(const void* p, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(p), "s"(dst) : "memory");
+}
+__device__ inline uint32_t lds_address(const void* p) {        // the same for the whole wavefront
+    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p);
+}
+// All but the wavefront's last N loads have arrived and its LDS reads are done; then everyone's.
+template <int N> __device__ inline void step_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// The tiles of a launch.  Workgroups are dealt to the eight dies in turn: each die takes one contiguous run of tiles, queries fastest
+// within a group, so that the tiles it works on at one time share rows and queries in its L2.
+struct TileOrder {
+    uint32_t row_tiles, q_tiles, q_group;
+    __device__ void at(uint64_t t, uint32_t& row_tile, uint32_t& q_tile) const {
+        const uint64_t whole = (uint64_t)row_tiles * q_group;
+        const uint32_t grp = (uint32_t)(t / whole), in_grp = min(q_group, q_tiles - grp * q_group);
+        const uint32_t left = (uint32_t)(t - grp * whole);
+        row_tile = left / in_grp; q_tile = grp * q_group + left % in_grp;
+    }
+};
+
+template <int BM, int BN, int WM, int WN, int S>
+__global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN))
+gemm_kernel(Q8View q, Q8View b, int metric, float* __restrict__ out, size_t out_stride, TileOrder order) {
+    constexpr int WAVES = (BM / WM) * (BN / WN), ROWS = BM + BN;
+    constexpr int KS = 64, CH = KS / 16, RPI = 64 / CH;        // columns per step, chunks per row, rows per load instruction of a wavefront
+    constexpr int LOADS = ROWS / (RPI * WAVES);                // load instructions per wavefront and step
+    constexpr int SLOADS = (ROWS / 64 + WAVES - 1) / WAVES;    // the same for the scales (a wavefront too many repeats the last one's)
+    constexpr int MT = WM / 32, NT = WN / 32;
+    typedef float Run __attribute__((ext_vector_type(MT)));
+    typedef Run UnalignedRun __attribute__((aligned(4)));
+    static_assert(ROWS % (RPI * WAVES) == 0 && BM % 64 == 0 && BN % 64 == 0 && S >= 3, "whole instructions");
+    __shared__ uint4 tile[S][ROWS * CH];
+    __shared__ uint32_t scale[S][ROWS];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), r = lane & 31, g = lane >> 5;
+
+    const uint64_t tiles = (uint64_t)order.row_tiles * order.q_tiles, per = (tiles + 7) / 8;
+    const uint64_t end = min((blockIdx.x % 8 + 1) * per, tiles);
+    uint64_t t = blockIdx.x % 8 * per + blockIdx.x / 8;        // the tile that is multiplied
+    if (t >= end) return;
+
+    // what this lane loads: chunk c of one row per instruction; rows behind the last repeat it (their results are not stored).
+    // Offsets count from the tile's first row: a tile is at most 256 rows of 2^24 bytes.
+    const uint32_t lr = lane / CH, c = (lane % CH) ^ (lr >> 2 & 3);
+    auto row_of = [](uint32_t slot) { return slot / WM * WM + MT * (slot % 32) + slot % WM / 32; };      // of the rows; a query's slot is its place
+    const uint32_t width = b.width(), steps = (width + KS - 1) / KS;
+    const uint32_t tile_dst = lds_address(&tile[0][wave * 64]);
+    uint32_t scale_dst[SLOADS];
+#pragma unroll
+    for (int i = 0; i < SLOADS; ++i) scale_dst[i] = lds_address(scale[0] + min(i * WAVES + wave, (uint32_t)ROWS / 64 - 1) * 64);
+    const uint8_t* row_base; const uint8_t* q_base;
+    uint32_t off[LOADS];
+    const uint8_t* scale_src[SLOADS];
+    auto load_from = [&](uint64_t at) {
+        uint32_t rt, qt;
+        order.at(at, rt, qt);
+        const uint32_t row0 = rt * BM, q0 = qt * BN;
+        row_base = b.codes + (size_t)row0 * b.cs; q_base = q.codes + (size_t)q0 * q.cs;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const uint32_t first = (i * WAVES + wave) * RPI;
+            off[i] = (first < BM ? min(row_of(first + lr), b.n - 1 - row0) * (uint32_t)b.cs : min(first - BM + lr, q.n - 1 - q0) * (uint32_t)q.cs) + c * 16;
+        }
+#pragma unroll
+        for (int i = 0; i < SLOADS; ++i) {
+            const uint32_t first = min(i * WAVES + wave, (uint32_t)ROWS / 64 - 1) * 64;
+            scale_src[i] = first < BM ? b.scales + (size_t)(row0 + min(row_of(first + lane), b.n - 1 - row0)) * b.ss : q.scales + (size_t)(q0 + min(first - BM + lane, q.n - 1 - q0)) * q.ss;
+        }
+    };
+    // The step that is loaded: fs of tile ft.  Behind the last tile its first steps come again and are not used: every step has the same
+    // number of loads.
+    uint64_t ft = t;
+    uint32_t fs = 0;
+    load_from(t);
+    auto fetch_tile = [&](uint32_t buf, int i) {
+        const uint32_t dst = tile_dst + buf * (ROWS * CH * 16) + i * (WAVES * 1024);
+        const uint8_t* base = ((i * WAVES + wave) * RPI < BM ? row_base : q_base) + (size_t)fs * KS;
+        if ((fs + 1) * KS <= width) load16_to_lds(base, off[i], dst);
+        else load16_to_lds(fs * KS + c * 16 < width ? (const void*)(base + off[i]) : (const void*)zero16, dst);      // zeros behind the rows' end
+    };
+    auto fetch_scales = [&](uint32_t buf) {
+#pragma unroll
+        for (int i = 0; i < SLOADS; ++i) load4_to_lds(scale_src[i] + (size_t)(fs / 8) * 4, scale_dst[i] + buf * (ROWS * 4));
+    };
+    auto fetched = [&] {
+        if (++fs < steps) return;
+        fs = 0;
+        ft += gridDim.x / 8;
+        if (ft < end) load_from(ft);
+    };
+
+    const uint32_t wm = wave % (BM / WM) * WM, wn = wave / (BM / WM) * WN;
+    floatx16 acc[MT][NT] = {};
+    struct Fragments { uint4 x[MT], y[NT]; };
+    Fragments f0, f1;
+    uint32_t xs[MT], ys[NT];
+    auto read = [&](Fragments& f, uint32_t buf, uint32_t h) {
+        const uint4* cur = tile[buf];
+        const uint32_t place = (2 * h + g) ^ (r >> 2 & 3);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) f.y[j] = cur[(BM + wn + 32 * j + r) * CH + place];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) f.x[i] = cur[(wm + 32 * i + r) * CH + place];
+    };
+    auto read_scales = [&](uint32_t buf) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) ys[j] = scale[buf][BM + wn + 32 * j + r];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) xs[i] = scale[buf][wm + 32 * i + r];
+    };
+    float xf[MT], yf[NT];
+    // One half step.  `slot(i)` comes between the products of row tiles i and i + 1: loads are spread over the step, because the
+    // wavefronts leave the barrier together and would otherwise queue for the memory pipe while the matrix pipe stands still.
+    auto multiply = [&](const Fragments& f, auto&& slot) {
+        bf16x8 y[NT][2], x[2][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) { y[j][0] = widen(f.y[j].x, f.y[j].y, yf[j]); y[j][1] = widen(f.y[j].z, f.y[j].w, yf[j]); }
+        x[0][0] = widen(f.x[0].x, f.x[0].y, xf[0]); x[0][1] = widen(f.x[0].z, f.x[0].w, xf[0]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            if (i + 1 < MT) { x[(i + 1) & 1][0] = widen(f.x[i + 1].x, f.x[i + 1].y, xf[i + 1]); x[(i + 1) & 1][1] = widen(f.x[i + 1].z, f.x[i + 1].w, xf[i + 1]); }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(y[j][h], x[i & 1][h], acc[i][j], 0, 0, 0);
+            slot(i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // Register e of tiles (0 .. MT - 1, j): rows row0 + MT r + 0 .. MT - 1 of query 32 j + 8 (e / 4) + 4 g + e mod 4.  Rows are asked
+    // for one by one only where the tile holds the last.  The stores need no more than the alignment of a float.
+    auto store_as = [&](auto kind, uint32_t row0, uint32_t q0) {
+        constexpr int METRIC = decltype(kind)::value;
+        const uint64_t row = (uint64_t)row0 + MT * r;
+        const bool whole = (uint64_t)row0 + WM <= b.n;
+        float nb[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) nb[i] = norm_of(b.norms2, min(row + i, (uint64_t)b.n - 1), METRIC);
+        float* lane_base = out + ((size_t)q0 + 4 * g) * out_stride + row;
+        const uint32_t left = q.n - 1 - q0;                    // the last query's place
+#pragma unroll
+        for (int e = 0; e < 16 * NT; e += 4) {                 // four queries at a time
+            float nq[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) nq[k] = norm_of(q.norms2, (size_t)q0 + min(2 * e + 4 * g + k, left), METRIC);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t at = 2 * e + k;
+                if (at + 4 * g > left) continue;
+                float* o = lane_base + (size_t)at * out_stride;
+                Run v;
+#pragma unroll
+                for (int i = 0; i < MT; ++i) v[i] = finish(acc[i][e / 16][e % 16 + k], nq[k], nb[i], METRIC);
+                if (whole) __builtin_nontemporal_store(v, reinterpret_cast<UnalignedRun*>(o));
+                else
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) if (row + i < b.n) o[i] = v[i];
+            }
+        }
+    };
+    auto store = [&] {
+        uint32_t rt, qt;
+        order.at(t, rt, qt);
+        const uint32_t row0 = rt * BM + wm, q0 = qt * BN + wn;
+        if (row0 < b.n && q0 < q.n) {
+            if (metric == VDB_DOT) store_as(std::integral_constant<int, VDB_DOT>{}, row0, q0);
+            else if (metric == VDB_COSINE) store_as(std::integral_constant<int, VDB_COSINE>{}, row0, q0);
+            else store_as(std::integral_constant<int, VDB_EUCLIDEAN>{}, row0, q0);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = floatx16{};
+    };
+
+    constexpr int PER = LOADS + SLOADS;
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) fetch_tile(s, i);
+        fetch_scales(s);
+        fetched();
+    }
+    step_barrier<(S - 2) * PER>();                             // the first step is there
+    read(f0, 0, 0); read_scales(0);
+    uint32_t buf = 0, s = 0;
+    while (true) {
+        step_barrier<(S - 3) * PER>();                         // the next step is there, and nobody reads the buffer of the last one any more
+        const uint32_t next = buf + 1 == S ? 0 : buf + 1, last = buf == 0 ? S - 1 : buf - 1, shift = 8 * (s >> 1 & 3);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) yf[j] = scale_of(ys[j] >> shift & 255u);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) xf[i] = scale_of(xs[i] >> shift & 255u);
+        read(f1, buf, 1);
+        __builtin_amdgcn_sched_barrier(0);                     // the reads stay ahead of the products that hide them
+        // 2 MT places for LOADS loads and the scales
+        constexpr int PLACES = 2 * MT, EACH = (LOADS + PLACES - 1) / PLACES;
+        multiply(f0, [&](int i) {
+#pragma unroll
+            for (int e = i * EACH; e < (i + 1) * EACH && e < LOADS; ++e) fetch_tile(last, e);
+        });
+        read(f0, next, 0); read_scales(next);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(f1, [&](int i) {
+#pragma unroll
+            for (int e = (MT + i) * EACH; e < (MT + i + 1) * EACH && e < LOADS; ++e) fetch_tile(last, e);
+            if (i == MT - 1) fetch_scales(last);
+        });
+        fetched();
+        buf = next;
+        if (++s < steps) continue;
+        s = 0;
+        store();
+        t += gridDim.x / 8;
+        if (t >= end) break;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // nothing lands in LDS behind the workgroup's end
 }
 
 // A wavefront scores 16 rows against 16 queries.
@@ -138,11 +393,11 @@ __global__ void __launch_bounds__(256) score_kernel(Q8View q, Q8View b, int metr
             }
         }
         if (q0 + r >= q.n) continue;
-        const float nq = metric == VDB_DOT ? 0.f : q.norms2[qu];
+        const float nq = norm_of(q.norms2, qu, metric);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t c = row0 + 4 * g + i;
-            if (c < b.n) out[(size_t)qu * out_stride + c] = finish(acc[i], nq, metric == VDB_DOT ? 0.f : b.norms2[c], metric);
+            if (c < b.n) out[(size_t)qu * out_stride + c] = finish(acc[i], nq, norm_of(b.norms2, c, metric), metric);
         }
     }
 }
@@ -160,7 +415,34 @@ void launch_q8_quantize(const void* rows, int dtype, size_t stride, const vdb_q8
     VDB_HIP(hipGetLastError());
 }
 
+static uint64_t tiles_of(uint32_t n, uint32_t size) { return ((uint64_t)n + size - 1) / size; }
+
+template <int BM, int BN, int WM, int WN, int S>
+static void launch_gemm(const Q8View& q, const Q8View& b, int metric, float* out, size_t out_stride, hipStream_t s) {
+    const uint32_t rt = (uint32_t)tiles_of(b.n, BM), qt = (uint32_t)tiles_of(q.n, BN);
+    constexpr int THREADS = 64 * (BM / WM) * (BN / WN);
+    static const int resident = [] {                           // workgroups the chip holds: every gfx950 device alike
+        int dev = 0, cus = 0, per_cu = 0;
+        VDB_HIP(hipGetDevice(&dev));
+        VDB_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
+        VDB_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, gemm_kernel<BM, BN, WM, WN, S>, THREADS, 0));
+        return std::max(cus * std::max(per_cu, 1), 8);
+    }();
+    const uint32_t grid = (uint32_t)std::min<uint64_t>(((uint64_t)rt * qt + 7) / 8, resident / 8) * 8;
+    hipLaunchKernelGGL((gemm_kernel<BM, BN, WM, WN, S>), dim3(grid), dim3(THREADS), 0, s, q, b, metric, out, out_stride, TileOrder{rt, qt, std::min<uint32_t>(qt, 2048 / BN)});
+    VDB_HIP(hipGetLastError());
+}
+
 void launch_q8_score(const Q8View& q, const Q8View& b, int metric, float* out, size_t out_stride, hipStream_t s) {
+    if (q.n > 16 && q.cs <= MAX_STRIDE && b.cs <= MAX_STRIDE) {
+        // The larger the tile, the fewer conversions and LDS reads per product (1000 x 1M x 960: 2.08 / 2.48 / 3.56 ms), but it has to be
+        // filled and there have to be enough of them: 77 x 300007 x 100 45.6 / 37.1 / 41.7 us, 64 x 1M x 960 452 / 306 / 292 us,
+        // 300 x 5000 x 768 27.2 / 17.8 / 12.0 us.
+        if (q.n > 128 && tiles_of(b.n, 256) * tiles_of(q.n, 256) >= 512) launch_gemm<256, 256, 128, 64, 4>(q, b, metric, out, out_stride, s);
+        else if (q.n > 64 && tiles_of(b.n, 256) * tiles_of(q.n, 128) >= 256) launch_gemm<256, 128, 64, 64, 4>(q, b, metric, out, out_stride, s);
+        else launch_gemm<128, 64, 64, 32, 4>(q, b, metric, out, out_stride, s);
+        return;
+    }
     const uint32_t row_tiles = (uint32_t)(((uint64_t)b.n + 15) / 16);
     const uint64_t tiles = (((uint64_t)q.n + 15) / 16) * row_tiles;
     const uint32_t blocks = (uint32_t)std::min<uint64_t>((tiles + 3) / 4, 1u << 20);
