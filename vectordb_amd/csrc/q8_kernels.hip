@@ -16,77 +16,113 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 // ---------------------------------------------------------------- quantiser
 // Block of 128 columns, a = max |x| over its finite values: e = the smallest exponent from -100 on with a <= 448 * 2^e, code =
 // e4m3(x * 2^-e) (v_cvt_pk_fp8_f32: nearest, ties to even; x * 2^-e is never beyond 448).  The smallest code is 2^-9: with e >= -100
-// every value held is an ordinary bf16 and f32 number; at e = 120 codes end at 240, so that no value rounds up to 2^128.  Half a wavefront holds a block, four columns per lane: the row is read once, codes leave 128 bytes at a time.
-// Bound by HBM: 4 (2) bytes read, 1 + 1/128 written per column.
+// every value held is an ordinary bf16 and f32 number; at e = 120 codes end at 240, so that no value rounds up to 2^128.
+// A lane reads 16 bytes, so 32 (16) lanes hold a block: a load reads 512 (256) bytes in a row, a store writes a whole line of codes.
+// Such a group walks through a row, and the next block is on its way while one is converted.
+// Bound by HBM: 4 (2) bytes read, 1 + 1/128 written per column.  1M x 960 f32 903 us = 5.3 TB/s (without the streaming hint on the codes
+// 918, with it on the rows too 1020; 16 lanes of 32 bytes 1040; two rows side by side 1058), 300007 x 100 bf16 29 us.
+
+constexpr size_t MAX_STRIDE = 1u << 24;     // of the rows that the tiled kernel takes: its offsets have 32 bits
+constexpr int MIN_EXP = -100, TOP_EXP = 120;
+
+template <int CTRL> __device__ inline uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true); }
+// Over the 16 lanes of a row: exchanges of neighbours, pairs, and two mirrors; over 32 across two rows.
+template <int LANES> __device__ inline uint32_t max_over(uint32_t v) {
+    v = max(v, dpp<0xB1>(v)); v = max(v, dpp<0x4E>(v)); v = max(v, dpp<0x141>(v)); v = max(v, dpp<0x140>(v));
+    if (LANES == 16) return v;
+    const auto w = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return max(w[0], w[1]);
+}
+template <int LANES> __device__ inline float sum_over(float v) {
+    v += __uint_as_float(dpp<0xB1>(__float_as_uint(v))); v += __uint_as_float(dpp<0x4E>(__float_as_uint(v)));
+    v += __uint_as_float(dpp<0x141>(__float_as_uint(v))); v += __uint_as_float(dpp<0x140>(__float_as_uint(v)));
+    if (LANES == 16) return v;
+    const auto w = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(w[0]) + __uint_as_float(w[1]);
+}
 
 __device__ inline float to_float(float v) { return v; }
 __device__ inline float to_float(_Float16 v) { return (float)v; }
 __device__ inline float to_float(__bf16 v) { return (float)v; }
 
-template <class T> struct alignas(4 * sizeof(T)) Four { T v[4]; };
-
-// `VEC`: row starts are aligned to four elements.
-template <class T, bool VEC> __device__ inline void load_four(const T* row, uint32_t k, uint32_t dim, float (&x)[4]) {
-    if (VEC && k + 4 <= dim) {
-        const Four<T> f = *reinterpret_cast<const Four<T>*>(row + k);
+// 16 bytes of a row, which need no more than the alignment of an element; zeros behind its end.
+template <class T> struct __attribute__((packed, aligned(sizeof(T)))) Piece { T v[16 / sizeof(T)]; };
+template <class T> __device__ inline Piece<T> load_piece(const T* row, uint32_t k, uint32_t dim) {
+    constexpr int E = 16 / sizeof(T);
+    if (k + E <= dim) return *reinterpret_cast<const Piece<T>*>(row + k);
+    Piece<T> f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = to_float(f.v[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = k + i < dim ? to_float(row[k + i]) : 0.f;
-    }
+    for (int i = 0; i < E; ++i) f.v[i] = k + i < dim ? row[k + i] : (T)0.f;
+    return f;
 }
 
-constexpr size_t MAX_STRIDE = 1u << 24;     // of the rows that the tiled kernel takes: its offsets have 32 bits
-constexpr int MIN_EXP = -100, TOP_EXP = 120;
-
-template <class T, bool VEC>
+template <class T>
 __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ rows, size_t stride, vdb_q8_rows out) {
-    const uint32_t lane = threadIdx.x & 31, dim = (uint32_t)out.dim;
+    constexpr int E = 16 / sizeof(T), LANES = Q8_BLOCK / E, GROUPS = 256 / LANES;
+    const uint32_t lane = threadIdx.x % LANES, dim = (uint32_t)out.dim;
     const uint32_t nb = (dim + Q8_BLOCK - 1) / Q8_BLOCK, width = (dim + 15u) & ~15u;
-    for (size_t r = (size_t)blockIdx.x * 8 + threadIdx.x / 32; r < out.n; r += (size_t)gridDim.x * 8) {
-        const T* row = rows + r * stride;
-        uint8_t* codes = out.codes + r * out.code_stride;
-        uint8_t* scales = out.scales + r * out.scale_stride;
-        float norm = 0.f;
-        for (uint32_t b = 0; b < nb; ++b) {
-            const uint32_t k = b * Q8_BLOCK + lane * 4;
-            float x[4];
-            load_four<T, VEC>(row, k, dim, x);
-            uint32_t a = 0;                                    // ordered as the absolute values are
+    const size_t all = (size_t)gridDim.x * GROUPS;
+    size_t r = (size_t)blockIdx.x * GROUPS + threadIdx.x / LANES, next_r = r;
+    if (r >= out.n) return;                                    // whole groups of lanes: the exchanges below stay within one
+    uint32_t b = 0, next_b = 0, scales = 0;
+    float norm = 0.f;
+    auto load = [&] {
+        const Piece<T> x = load_piece(rows + next_r * stride, next_b * Q8_BLOCK + lane * E, dim);
+        if (++next_b < nb) return x;
+        next_b = 0;
+        if (out.n - next_r > all) next_r += all;               // behind the last row it comes again and is not used
+        return x;
+    };
+    Piece<T> next = load();
+    while (true) {
+        float x[E];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t u = __float_as_uint(x[i]) & 0x7FFFFFFFu;
-                if (u < 0x7F800000u) a = max(a, u);
-            }
+        for (int i = 0; i < E; ++i) x[i] = to_float(next.v[i]);
+        next = load();
+        uint32_t a = 0;                                        // ordered as the absolute values are
 #pragma unroll
-            for (int o = 16; o; o >>= 1) a = max(a, (uint32_t)__shfl_xor((int)a, o, 64));
-            // a = m * 2^E with 1 <= m < 2, 448 = 1.75 * 2^8
-            int e = (int)(a >> 23) - 127 - 8 + ((a & 0x7FFFFFu) > 0x600000u);
-            e = a == 0 ? 0 : max(e, MIN_EXP);
-            const float up = __uint_as_float((uint32_t)(127 - e) << 23), down = __uint_as_float((uint32_t)(127 + e) << 23);
-            const float top = e == TOP_EXP ? 240.f : 448.f;
-            uint32_t c = 0;
+        for (int i = 0; i < E; ++i) {
+            const uint32_t v = __float_as_uint(x[i]) & 0x7FFFFFFFu;
+            a = max(a, v < 0x7F800000u ? v : 0u);
+        }
+        a = max_over<LANES>(a);
+        // a = m * 2^E with 1 <= m < 2, 448 = 1.75 * 2^8
+        int e = (int)(a >> 23) - 127 - 8 + ((a & 0x7FFFFFu) > 0x600000u);
+        e = a == 0 ? 0 : max(e, MIN_EXP);
+        const float up = __uint_as_float((uint32_t)(127 - e) << 23), down = __uint_as_float((uint32_t)(127 + e) << 23);
+        const float top = e == TOP_EXP ? 240.f : 448.f;
+        typedef uint32_t Codes __attribute__((ext_vector_type(E / 4)));
+        Codes c;
+#pragma unroll
+        for (int h = 0; h < E / 4; ++h) {
             float y[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_fmed3f(x[i] * up, -top, top);
-            c = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], c, false);
-            c = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c, true);
+            for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_fmed3f(x[4 * h + i] * up, -top, top);
+            uint32_t w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+            w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) if ((__float_as_uint(x[i]) & 0x7FFFFFFFu) >= 0x7F800000u) c = (c & ~(0xFFu << (8 * i))) | (0x7Fu << (8 * i));
-            const float v0 = __builtin_amdgcn_cvt_f32_fp8(c, 0) * down, v1 = __builtin_amdgcn_cvt_f32_fp8(c, 1) * down;
-            const float v2 = __builtin_amdgcn_cvt_f32_fp8(c, 2) * down, v3 = __builtin_amdgcn_cvt_f32_fp8(c, 3) * down;
+            for (int i = 0; i < 4; ++i) if ((__float_as_uint(x[4 * h + i]) & 0x7FFFFFFFu) >= 0x7F800000u) w = (w & ~(0xFFu << (8 * i))) | (0x7Fu << (8 * i));
+            const float v0 = __builtin_amdgcn_cvt_f32_fp8(w, 0) * down, v1 = __builtin_amdgcn_cvt_f32_fp8(w, 1) * down;
+            const float v2 = __builtin_amdgcn_cvt_f32_fp8(w, 2) * down, v3 = __builtin_amdgcn_cvt_f32_fp8(w, 3) * down;
             norm = __builtin_fmaf(v0, v0, norm); norm = __builtin_fmaf(v1, v1, norm);
             norm = __builtin_fmaf(v2, v2, norm); norm = __builtin_fmaf(v3, v3, norm);
-            if (k < width) *reinterpret_cast<uint32_t*>(codes + k) = c;
-            if (lane == 0) scales[b] = (uint8_t)(e + 127);
+            c[h] = w;
         }
-        if (lane < ((nb + 3) & ~3u) - nb) scales[nb + lane] = 127;
+        const uint32_t k = b * Q8_BLOCK + lane * E;
+        if (k < width) __builtin_nontemporal_store(c, reinterpret_cast<Codes*>(out.codes + r * out.code_stride + k));
+        if (b % 4 == 0) scales = 0x7F7F7F7Fu;                  // blocks behind the last: 127
+        scales = (scales & ~(0xFFu << (8 * (b % 4)))) | (uint32_t)(e + 127) << (8 * (b % 4));
+        const bool last = b + 1 == nb;
+        if (lane == 0 && (last || b % 4 == 3)) *reinterpret_cast<uint32_t*>(out.scales + r * out.scale_stride + b / 4 * 4) = scales;
+        ++b;
+        if (!last) continue;
         if (out.norms2) {
-#pragma unroll
-            for (int o = 16; o; o >>= 1) norm += __shfl_xor(norm, o, 64);
+            norm = sum_over<LANES>(norm);
             if (lane == 0) out.norms2[r] = norm;
         }
+        b = 0; norm = 0.f;
+        if (out.n - r <= all) return;
+        r += all;
     }
 }
 
@@ -373,6 +409,111 @@ gemm_kernel(Q8View q, Q8View b, int metric, float* __restrict__ out, size_t out_
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // nothing lands in LDS behind the workgroup's end
 }
 
+// Up to 16 queries: bound by the pass over the rows, which go from memory to registers.  The queries' codes lie in LDS, 16-byte chunk
+// by chunk.  A wavefront takes 16 rows at a time, a block of 128 columns a step, and has the next step's codes on their way while it
+// multiplies one.  The queries are the left operand: a result register holds 16 rows of four queries.
+// Measured on 1 x 1M x 960: 171 us = 5.7 TB/s (8 queries 201 us); four blocks a step 166 us there and 113 instead of 109 us on 300000 x
+// 2048; 64 rows at a time 190 .. 212 us; with the streaming hint 190 us (the second half of a line is fetched again).
+// SPLIT: the four wavefronts of a workgroup take a quarter of the columns each of the same rows and add up in LDS, in one order.
+template <bool SPLIT>
+__global__ void __launch_bounds__(256) stream_kernel(Q8View q, Q8View b, int metric, float* __restrict__ out, size_t out_stride, uint32_t groups) {
+    extern __shared__ uint4 query[];                           // [8 chunks per block][16 queries], then the scales [4 blocks][16]
+    __shared__ floatx4 part[3][SPLIT ? 64 : 1];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), r = lane & 15, g = lane >> 4;
+    const uint32_t nb = b.blocks(), width = b.width();
+    uint32_t* query_scale = reinterpret_cast<uint32_t*>(query + nb * 128);
+    for (uint32_t i = threadIdx.x; i < nb * 128; i += 256) query[i] = load16(q.codes + (size_t)min(i % 16, q.n - 1) * q.cs, i / 16 * 16, width);
+    for (uint32_t i = threadIdx.x; i < (nb + 3) / 4 * 16; i += 256) query_scale[i] = *reinterpret_cast<const uint32_t*>(q.scales + (size_t)min(i % 16, q.n - 1) * q.ss + i / 16 * 4);
+    __syncthreads();
+    float nq[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) nq[e] = norm_of(q.norms2, min(4 * g + e, q.n - 1), metric);
+
+    const uint32_t first_group = SPLIT ? blockIdx.x : blockIdx.x * 4 + wave, stride = SPLIT ? gridDim.x : gridDim.x * 4;
+    if (first_group >= groups) return;                         // SPLIT: of the whole workgroup
+    struct Step { uint4 v[2]; uint32_t scale; };
+    const uint8_t* row; const uint8_t* row_scales;
+    auto go_to = [&](uint32_t group) {                         // rows behind the last repeat it; they are not stored
+        const size_t i = min((uint64_t)group * 16 + r, (uint64_t)b.n - 1);
+        row = b.codes + i * b.cs + 16 * g;
+        row_scales = b.scales + i * b.ss;
+    };
+    auto load = [&](Step& to, uint32_t k) {
+        to.scale = row_scales[k];
+        const uint32_t at = k * Q8_BLOCK;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) to.v[h] = at + 64 * h + 16 * g < width ? *reinterpret_cast<const uint4*>(row + at + 64 * h) : uint4{0, 0, 0, 0};
+    };
+    floatx4 acc{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const Step& x, uint32_t k) {
+        const float qs = scale_of(query_scale[k / 4 * 16 + r] >> (8 * (k & 3)) & 255u), rs = scale_of(x.scale);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint4 v = query[(k * 8 + 4 * h + g) * 16 + r], w = x.v[h];
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(v.x, v.y, qs), widen(w.x, w.y, rs), acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(v.z, v.w, qs), widen(w.z, w.w, rs), acc, 0, 0, 0);
+        }
+    };
+    auto store = [&](uint32_t group) {
+        const uint64_t i = (uint64_t)group * 16 + r;
+        if (i >= b.n) return;
+        const float norm = norm_of(b.norms2, i, metric);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (4 * g + e < q.n) out[(size_t)(4 * g + e) * out_stride + i] = finish(acc[e], nq[e], norm, metric);
+    };
+    Step x, y;
+
+    if (SPLIT) {
+        const uint32_t lo = nb * wave / 4, hi = nb * (wave + 1) / 4;
+        for (uint32_t group = first_group; group < groups; group += stride) {
+            go_to(group);
+            acc = floatx4{0.f, 0.f, 0.f, 0.f};
+            if (lo < hi) load(x, lo);
+            for (uint32_t k = lo; k < hi; k += 2) {
+                load(y, min(k + 1, hi - 1));
+                multiply(x, k);
+                if (k + 1 >= hi) break;
+                load(x, min(k + 2, hi - 1));
+                multiply(y, k + 1);
+            }
+            __syncthreads();                                   // the parts of the last group are read
+            if (wave) part[wave - 1][lane] = acc;
+            __syncthreads();
+            if (wave) continue;
+#pragma unroll
+            for (int w = 0; w < 3; ++w) acc += part[w][lane];
+            store(group);
+        }
+        return;
+    }
+    // the blocks of all groups in one sequence
+    uint32_t group = first_group, k = 0, next_group = first_group, next_k = 0;
+    auto load_next = [&](Step& to) {
+        load(to, next_k);
+        if (++next_k < nb) return;
+        next_k = 0;
+        if (groups - next_group > stride) { next_group += stride; go_to(next_group); }     // behind the last group it comes again and is not used
+    };
+    auto take = [&](const Step& x) {                           // -> whether the last group is done
+        multiply(x, k);
+        if (++k < nb) return false;
+        k = 0;
+        store(group);
+        acc = floatx4{0.f, 0.f, 0.f, 0.f};
+        if (groups - group <= stride) return true;
+        group += stride;
+        return false;
+    };
+    go_to(group);
+    load_next(x);
+    while (true) {
+        load_next(y);
+        if (take(x)) return;
+        load_next(x);
+        if (take(y)) return;
+    }
+}
+
 // A wavefront scores 16 rows against 16 queries.
 __global__ void __launch_bounds__(256) score_kernel(Q8View q, Q8View b, int metric, float* __restrict__ out, size_t out_stride, uint32_t row_tiles, uint64_t tiles) {
     const uint32_t lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
@@ -404,15 +545,19 @@ __global__ void __launch_bounds__(256) score_kernel(Q8View q, Q8View b, int metr
 
 }  // namespace
 
-void launch_q8_quantize(const void* rows, int dtype, size_t stride, const vdb_q8_rows& out, hipStream_t s) {
-    const uint32_t blocks = (uint32_t)std::min<size_t>((out.n + 7) / 8, 1u << 20);
-    const size_t size = dtype == VDB_F32 ? 4 : 2;
-    const bool vec = (uintptr_t)rows % (4 * size) == 0 && stride % 4 == 0;
-#define VDB_QUANT(T) do { if (vec) hipLaunchKernelGGL((quantize_kernel<T, true>), dim3(blocks), dim3(256), 0, s, (const T*)rows, stride, out); \
-                          else hipLaunchKernelGGL((quantize_kernel<T, false>), dim3(blocks), dim3(256), 0, s, (const T*)rows, stride, out); } while (0)
-    if (dtype == VDB_F32) VDB_QUANT(float); else if (dtype == VDB_F16) VDB_QUANT(_Float16); else VDB_QUANT(__bf16);
-#undef VDB_QUANT
+template <class T> static void launch_quantize(const T* rows, size_t stride, const vdb_q8_rows& out, hipStream_t s) {
+    constexpr size_t per = 256 / (Q8_BLOCK / (16 / sizeof(T)));
+    // A group per row while the grid allows (1M x 960: 911 us; 8192 workgroups that walk on 993, 2048 1018), but rows of one block are over
+    // too soon for that (1M x 128: 142 against 130 us, 300007 x 100 bf16: 31.5 against 29.1).
+    const uint32_t blocks = (uint32_t)std::min<size_t>((out.n + per - 1) / per, out.dim <= Q8_BLOCK ? 8192 : 1u << 18);
+    hipLaunchKernelGGL(quantize_kernel<T>, dim3(blocks), dim3(256), 0, s, rows, stride, out);
     VDB_HIP(hipGetLastError());
+}
+
+void launch_q8_quantize(const void* rows, int dtype, size_t stride, const vdb_q8_rows& out, hipStream_t s) {
+    if (dtype == VDB_F32) launch_quantize((const float*)rows, stride, out, s);
+    else if (dtype == VDB_F16) launch_quantize((const _Float16*)rows, stride, out, s);
+    else launch_quantize((const __bf16*)rows, stride, out, s);
 }
 
 static uint64_t tiles_of(uint32_t n, uint32_t size) { return ((uint64_t)n + size - 1) / size; }
@@ -434,13 +579,24 @@ static void launch_gemm(const Q8View& q, const Q8View& b, int metric, float* out
 }
 
 void launch_q8_score(const Q8View& q, const Q8View& b, int metric, float* out, size_t out_stride, hipStream_t s) {
-    if (q.n > 16 && q.cs <= MAX_STRIDE && b.cs <= MAX_STRIDE) {
+    if ((q.n > 16 || b.width() > 4096) && q.cs <= MAX_STRIDE && b.cs <= MAX_STRIDE) {
         // The larger the tile, the fewer conversions and LDS reads per product (1000 x 1M x 960: 2.08 / 2.48 / 3.56 ms), but it has to be
         // filled and there have to be enough of them: 77 x 300007 x 100 45.6 / 37.1 / 41.7 us, 64 x 1M x 960 452 / 306 / 292 us,
         // 300 x 5000 x 768 27.2 / 17.8 / 12.0 us.
         if (q.n > 128 && tiles_of(b.n, 256) * tiles_of(q.n, 256) >= 512) launch_gemm<256, 256, 128, 64, 4>(q, b, metric, out, out_stride, s);
         else if (q.n > 64 && tiles_of(b.n, 256) * tiles_of(q.n, 128) >= 256) launch_gemm<256, 128, 64, 64, 4>(q, b, metric, out, out_stride, s);
         else launch_gemm<128, 64, 64, 32, 4>(q, b, metric, out, out_stride, s);
+        return;
+    }
+    if (q.n <= 16 && b.width() <= 4096) {                      // 64 KiB of LDS for the queries
+        const uint32_t nb = b.blocks(), groups = (uint32_t)tiles_of(b.n, 16);
+        const size_t lds = (size_t)nb * 2048 + (nb + 3) / 4 * 64;
+        // Few rows: a workgroup per 16 of them (kernel times: 10064 x 960 5.6 against 6.4 us, 2000 x 4096 8.5 against 15.5, but 100000 x 960
+        // 20.9 against 19.4).  The resident workgroups walk through the rest: 1M rows of 128 / 256 / 960 columns on 1024 workgroups 24.5 /
+        // 38.7 / 171 us, on 2048 23.1 / 41.0 / 187.
+        if (groups <= 2048 && nb >= 4) hipLaunchKernelGGL(stream_kernel<true>, dim3(groups), dim3(256), lds, s, q, b, metric, out, out_stride, groups);
+        else hipLaunchKernelGGL(stream_kernel<false>, dim3(std::min((groups + 3) / 4, nb == 1 ? 2048u : 1024u)), dim3(256), lds, s, q, b, metric, out, out_stride, groups);
+        VDB_HIP(hipGetLastError());
         return;
     }
     const uint32_t row_tiles = (uint32_t)(((uint64_t)b.n + 15) / 16);
