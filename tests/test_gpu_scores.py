@@ -1,7 +1,7 @@
 """8-bit rows, their block-scaled product and score rows on the GPU, against plain 64-bit forms.
 
 Tolerances count roundings (u = 2^-24, half a step of f32):
-  norms2    a lane's chain of at most 8 per block and 5 exchanges of non-negative terms: (8 blocks + 5) u of the sum
+  norms2    a lane's chain of at most 8 per block, 5 exchanges and 15 further sums of non-negative terms: (8 blocks + 20) u of the sum
   dot       exact products; one rounding of at most a whole step (2 u) per addition: 2 u 128 blocks of sum |q_i r_i|
   cosine    that over |q||r|, and eight roundings of values no larger than 1 + |cos|
   euclidean the square: twice the dot's, and four roundings of |q|^2 + |r|^2; the root: one step more
@@ -86,7 +86,7 @@ def check_scores(got, q, b, metric, dim):
     dot, mag = q @ b.T, np.abs(q) @ np.abs(b).T
     off = 2 * U * 128 * -(-dim // 128) * mag
     nq, nb = (q * q).sum(1)[:, None], (b * b).sum(1)[None]
-    norm_off = (8 * -(-dim // 128) + 5) * U
+    norm_off = (8 * -(-dim // 128) + 20) * U
     if metric == M.Dot:
         assert np.all(np.abs(got - dot) <= off + 2.0 ** -149)
     elif metric == M.Cosine:
@@ -106,7 +106,7 @@ def gauss(n, dim, seed, spread=2.0):
 # ---------------------------------------------------------------- quantiser
 
 @pytest.mark.parametrize("kind", list(TYPES))
-@pytest.mark.parametrize("n,dim", [(1, 1), (3, 3), (9, 16), (5, 17), (33, 100), (8, 127), (7, 128), (17, 129), (2, 511), (3, 513), (6, 960), (2, 4100)])
+@pytest.mark.parametrize("n,dim", [(1, 1), (3, 3), (9, 16), (5, 17), (33, 100), (8, 127), (7, 128), (17, 129), (2, 511), (3, 513), (6, 960), (2, 4100), (600, 300), (2049, 260), (2200, 129), (700, 90)])
 def test_quantised_rows_equal_the_definition(vdb, kind, n, dim):
     x = gauss(n, dim, n * 1000 + dim).to(TYPES[kind])
     r = S.quantize_rows(x.cuda())
@@ -114,7 +114,7 @@ def test_quantised_rows_equal_the_definition(vdb, kind, n, dim):
     assert np.array_equal(r.codes.cpu().numpy(), codes)
     assert np.array_equal(r.scales.cpu().numpy(), scales)
     want = (vals * vals).sum(1)
-    assert np.all(np.abs(r.norms2.cpu().numpy() - want) <= (8 * -(-dim // 128) + 5) * U * want)
+    assert np.all(np.abs(r.norms2.cpu().numpy() - want) <= (8 * -(-dim // 128) + 20) * U * want)
 
 
 def test_special_values(vdb):

@@ -56,9 +56,48 @@ template <class T> __device__ inline Piece<T> load_piece(const T* row, uint32_t 
     return f;
 }
 
+// What a group of lanes makes of a block: a lane's codes, the exponent, and the lane's share of the squared norm.
+template <class T> struct Coded {
+    static constexpr int E = 16 / sizeof(T), LANES = Q8_BLOCK / E;
+    typedef uint32_t Codes __attribute__((ext_vector_type(E / 4)));
+    Codes c;
+    int e;
+    __device__ Coded(const Piece<T>& in, float& norm) {
+        float x[E];
+        uint32_t a = 0;                                        // ordered as the absolute values are
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            x[i] = to_float(in.v[i]);
+            const uint32_t v = __float_as_uint(x[i]) & 0x7FFFFFFFu;
+            a = max(a, v < 0x7F800000u ? v : 0u);
+        }
+        a = max_over<LANES>(a);
+        // a = m * 2^E with 1 <= m < 2, 448 = 1.75 * 2^8
+        e = (int)(a >> 23) - 127 - 8 + ((a & 0x7FFFFFu) > 0x600000u);
+        e = a == 0 ? 0 : max(e, MIN_EXP);
+        const float up = __uint_as_float((uint32_t)(127 - e) << 23), down = __uint_as_float((uint32_t)(127 + e) << 23);
+        const float top = e == TOP_EXP ? 240.f : 448.f;
+#pragma unroll
+        for (int h = 0; h < E / 4; ++h) {
+            float y[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_fmed3f(x[4 * h + i] * up, -top, top);
+            uint32_t w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+            w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) if ((__float_as_uint(x[4 * h + i]) & 0x7FFFFFFFu) >= 0x7F800000u) w = (w & ~(0xFFu << (8 * i))) | (0x7Fu << (8 * i));
+            const float v0 = __builtin_amdgcn_cvt_f32_fp8(w, 0) * down, v1 = __builtin_amdgcn_cvt_f32_fp8(w, 1) * down;
+            const float v2 = __builtin_amdgcn_cvt_f32_fp8(w, 2) * down, v3 = __builtin_amdgcn_cvt_f32_fp8(w, 3) * down;
+            norm = __builtin_fmaf(v0, v0, norm); norm = __builtin_fmaf(v1, v1, norm);
+            norm = __builtin_fmaf(v2, v2, norm); norm = __builtin_fmaf(v3, v3, norm);
+            c[h] = w;
+        }
+    }
+};
+
 template <class T>
 __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ rows, size_t stride, vdb_q8_rows out) {
-    constexpr int E = 16 / sizeof(T), LANES = Q8_BLOCK / E, GROUPS = 256 / LANES;
+    constexpr int E = Coded<T>::E, LANES = Coded<T>::LANES, GROUPS = 256 / LANES;
     const uint32_t lane = threadIdx.x % LANES, dim = (uint32_t)out.dim;
     const uint32_t nb = (dim + Q8_BLOCK - 1) / Q8_BLOCK, width = (dim + 15u) & ~15u;
     const size_t all = (size_t)gridDim.x * GROUPS;
@@ -75,43 +114,13 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ row
     };
     Piece<T> next = load();
     while (true) {
-        float x[E];
-#pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = to_float(next.v[i]);
+        const Piece<T> x = next;
         next = load();
-        uint32_t a = 0;                                        // ordered as the absolute values are
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const uint32_t v = __float_as_uint(x[i]) & 0x7FFFFFFFu;
-            a = max(a, v < 0x7F800000u ? v : 0u);
-        }
-        a = max_over<LANES>(a);
-        // a = m * 2^E with 1 <= m < 2, 448 = 1.75 * 2^8
-        int e = (int)(a >> 23) - 127 - 8 + ((a & 0x7FFFFFu) > 0x600000u);
-        e = a == 0 ? 0 : max(e, MIN_EXP);
-        const float up = __uint_as_float((uint32_t)(127 - e) << 23), down = __uint_as_float((uint32_t)(127 + e) << 23);
-        const float top = e == TOP_EXP ? 240.f : 448.f;
-        typedef uint32_t Codes __attribute__((ext_vector_type(E / 4)));
-        Codes c;
-#pragma unroll
-        for (int h = 0; h < E / 4; ++h) {
-            float y[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_fmed3f(x[4 * h + i] * up, -top, top);
-            uint32_t w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-            w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) if ((__float_as_uint(x[4 * h + i]) & 0x7FFFFFFFu) >= 0x7F800000u) w = (w & ~(0xFFu << (8 * i))) | (0x7Fu << (8 * i));
-            const float v0 = __builtin_amdgcn_cvt_f32_fp8(w, 0) * down, v1 = __builtin_amdgcn_cvt_f32_fp8(w, 1) * down;
-            const float v2 = __builtin_amdgcn_cvt_f32_fp8(w, 2) * down, v3 = __builtin_amdgcn_cvt_f32_fp8(w, 3) * down;
-            norm = __builtin_fmaf(v0, v0, norm); norm = __builtin_fmaf(v1, v1, norm);
-            norm = __builtin_fmaf(v2, v2, norm); norm = __builtin_fmaf(v3, v3, norm);
-            c[h] = w;
-        }
+        const Coded<T> coded(x, norm);
         const uint32_t k = b * Q8_BLOCK + lane * E;
-        if (k < width) __builtin_nontemporal_store(c, reinterpret_cast<Codes*>(out.codes + r * out.code_stride + k));
+        if (k < width) __builtin_nontemporal_store(coded.c, reinterpret_cast<typename Coded<T>::Codes*>(out.codes + r * out.code_stride + k));
         if (b % 4 == 0) scales = 0x7F7F7F7Fu;                  // blocks behind the last: 127
-        scales = (scales & ~(0xFFu << (8 * (b % 4)))) | (uint32_t)(e + 127) << (8 * (b % 4));
+        scales = (scales & ~(0xFFu << (8 * (b % 4)))) | (uint32_t)(coded.e + 127) << (8 * (b % 4));
         const bool last = b + 1 == nb;
         if (lane == 0 && (last || b % 4 == 3)) *reinterpret_cast<uint32_t*>(out.scales + r * out.scale_stride + b / 4 * 4) = scales;
         ++b;
@@ -124,6 +133,35 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ row
         if (out.n - r <= all) return;
         r += all;
     }
+}
+
+// Few rows: a workgroup per row, its blocks side by side.
+template <class T>
+__global__ void __launch_bounds__(256) quantize_row_kernel(const T* __restrict__ rows, size_t stride, vdb_q8_rows out) {
+    constexpr int E = Coded<T>::E, LANES = Coded<T>::LANES, GROUPS = 256 / LANES;
+    __shared__ float part[GROUPS];
+    const uint32_t lane = threadIdx.x % LANES, group = threadIdx.x / LANES, dim = (uint32_t)out.dim;
+    const uint32_t nb = (dim + Q8_BLOCK - 1) / Q8_BLOCK, width = (dim + 15u) & ~15u;
+    const size_t r = blockIdx.x;
+    float norm = 0.f;
+    for (uint32_t b = group; b < ((nb + 3) & ~3u); b += GROUPS) {
+        if (b >= nb) {                                         // blocks behind the last: 127
+            if (lane == 0) out.scales[r * out.scale_stride + b] = 127;
+            continue;
+        }
+        const uint32_t k = b * Q8_BLOCK + lane * E;
+        const Coded<T> coded(load_piece(rows + r * stride, k, dim), norm);
+        if (k < width) *reinterpret_cast<typename Coded<T>::Codes*>(out.codes + r * out.code_stride + k) = coded.c;
+        if (lane == 0) out.scales[r * out.scale_stride + b] = (uint8_t)(coded.e + 127);
+    }
+    norm = sum_over<LANES>(norm);
+    if (lane == 0) part[group] = norm;
+    __syncthreads();
+    if (threadIdx.x || !out.norms2) return;
+    norm = 0.f;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) norm += part[i];
+    out.norms2[r] = norm;
 }
 
 // ---------------------------------------------------------------- block-scaled product
@@ -546,7 +584,14 @@ __global__ void __launch_bounds__(256) score_kernel(Q8View q, Q8View b, int metr
 }  // namespace
 
 template <class T> static void launch_quantize(const T* rows, size_t stride, const vdb_q8_rows& out, hipStream_t s) {
-    constexpr size_t per = 256 / (Q8_BLOCK / (16 / sizeof(T)));
+    // Kernel times for 1 / 500 / 2000 / 4000 rows of 960: 1.8 / 2.8 / 4.1 / 5.8 us a workgroup per row, 4.8 / 6.1 / 6.4 / 7.1 a group of lanes
+    // per row; 4000 x 256: 4.1 against 3.3.
+    if (out.n <= 2048 && out.dim > Q8_BLOCK) {
+        hipLaunchKernelGGL(quantize_row_kernel<T>, dim3((uint32_t)out.n), dim3(256), 0, s, rows, stride, out);
+        VDB_HIP(hipGetLastError());
+        return;
+    }
+    constexpr size_t per = 256 / Coded<T>::LANES;
     // A group per row while the grid allows (1M x 960: 911 us; 8192 workgroups that walk on 993, 2048 1018), but rows of one block are over
     // too soon for that (1M x 128: 142 against 130 us, 300007 x 100 bf16: 31.5 against 29.1).
     const uint32_t blocks = (uint32_t)std::min<size_t>((out.n + per - 1) / per, out.dim <= Q8_BLOCK ? 8192 : 1u << 18);

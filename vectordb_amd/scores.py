@@ -22,13 +22,19 @@ _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _METRICS = frozenset(int(m) for m in DistanceMetric)
 
 
+_lib = None
+
+
 def _api():
-    from . import api
-    return api()
+    global _lib
+    if _lib is None:
+        from . import api
+        _lib = api()
+    return _lib
 
 
-def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
+# the handle alone, without a Stream object around it (2 us a call), where torch offers it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _refuse(why):
@@ -37,37 +43,42 @@ def _refuse(why):
 
 def _check(t, what, dtype, ndim, device=None):
     """A tensor of one type and rank whose last axis is dense; -> elements from row to row."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != ndim:
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.dim() != ndim:
         _refuse(f"{what}: expected a {ndim}-d {dtype} tensor")
     if device is not None and t.device != device:
         _refuse(f"{what} is on {t.device}, not on {device}")
-    if not t.numel():
-        return t.shape[-1]
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    shape, stride = t.shape, t.stride()
+    width = shape[-1]
+    if ndim == 2:
+        n = shape[0]
+        if n and width:
+            if width > 1 and stride[1] != 1:
+                _refuse(f"{what}: the last axis must be dense")
+            if n > 1:
+                if stride[0] < width:
+                    _refuse(f"{what}: rows overlap")
+                return stride[0]
+    elif width > 1 and stride[0] != 1:
         _refuse(f"{what}: the last axis must be dense")
-    if ndim == 2 and t.shape[0] > 1:
-        if t.stride(0) < t.shape[1]:
-            _refuse(f"{what}: rows overlap")
-        return t.stride(0)
-    return t.shape[-1]
+    return width
 
 
 def _on_gpu(t, what):
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         _refuse(f"{what} must be a tensor on the GPU")
 
 
 def _metric(m):
-    if int(m) not in _METRICS:
+    if m not in _METRICS:
         _refuse("unknown metric")
     return int(m)
 
 
 def _out(out, nq, n, device):
     if out is None:
-        return torch.empty(nq, n, dtype=torch.float32, device=device), n
+        return torch.empty((nq, n), dtype=torch.float32, device=device), n
     stride = _check(out, "out", torch.float32, 2, device)
-    if tuple(out.shape) != (nq, n):
+    if out.shape != (nq, n):
         _refuse(f"out: expected shape {(nq, n)}")
     return out, stride
 
@@ -79,18 +90,21 @@ class Q8Rows:
 
     def __init__(self, codes, scales, norms2, dim):
         _on_gpu(codes, "codes")
-        cs, ss = _check(codes, "codes", torch.uint8, 2), _check(scales, "scales", torch.uint8, 2, codes.device)
-        n, dim = codes.shape[0], int(dim)
-        if dim < 1 or codes.shape[1] < -(-dim // 16) * 16 or scales.shape[1] < -(-dim // (4 * BLOCK)) * 4:
+        dev = codes.device
+        cs, ss = _check(codes, "codes", torch.uint8, 2), _check(scales, "scales", torch.uint8, 2, dev)
+        (n, wide), (m, blocks), dim = codes.shape, scales.shape, int(dim)
+        if dim < 1 or wide < -(-dim // 16) * 16 or blocks < -(-dim // (4 * BLOCK)) * 4:
             _refuse("codes or scales are narrower than a row")
-        if scales.shape[0] != n:
+        if m != n:
             _refuse("codes and scales hold different numbers of rows")
+        norms = None
         if norms2 is not None:
-            _check(norms2, "norms2", torch.float32, 1, codes.device)
+            _check(norms2, "norms2", torch.float32, 1, dev)
             if norms2.shape[0] != n:
                 _refuse("codes and norms2 hold different numbers of rows")
+            norms = norms2.data_ptr()
         self.codes, self.scales, self.norms2, self.dim = codes, scales, norms2, dim
-        self._c = Q8RowsC(codes.data_ptr(), scales.data_ptr(), norms2.data_ptr() if norms2 is not None else None, n, dim, cs, ss)
+        self._c = Q8RowsC(codes.data_ptr(), scales.data_ptr(), norms, n, dim, cs, ss)
 
     @classmethod
     def empty(cls, n, dim, device):
@@ -98,8 +112,12 @@ class Q8Rows:
         if dim < 1 or n < 0:
             _refuse("empty rows")
         wide, blocks = -(-dim // 16) * 16, -(-dim // (4 * BLOCK)) * 4
-        return cls(torch.empty(n, wide, dtype=torch.uint8, device=device), torch.empty(n, blocks, dtype=torch.uint8, device=device),
-                   torch.empty(n, dtype=torch.float32, device=device), dim)
+        self = cls.__new__(cls)
+        self.codes, self.scales = torch.empty((n, wide), dtype=torch.uint8, device=device), torch.empty((n, blocks), dtype=torch.uint8, device=device)
+        self.norms2, self.dim = torch.empty(n, dtype=torch.float32, device=device), dim
+        _on_gpu(self.codes, "a Q8Rows")
+        self._c = Q8RowsC(self.codes.data_ptr(), self.scales.data_ptr(), self.norms2.data_ptr(), n, dim, wide, blocks)
+        return self
 
     def __len__(self):
         return self.codes.shape[0]
@@ -114,16 +132,17 @@ class Q8Rows:
 def quantize_rows(rows, out=None):
     """f32 / f16 / bf16 rows [n, dim] -> Q8Rows (into `out` where given: appending is quantize_rows(new, out=room[n:n + k]))."""
     _on_gpu(rows, "rows")
-    if rows.dtype not in _DTYPES:
+    kind = _DTYPES.get(rows.dtype)
+    if kind is None:
         _refuse("rows: expected f32, f16 or bf16")
     stride = _check(rows, "rows", rows.dtype, 2)
-    n, dim = rows.shape
+    (n, dim), dev = rows.shape, rows.device
     if out is None:
-        out = Q8Rows.empty(n, dim, rows.device)
-    elif len(out) != n or out.dim != dim or out.codes.device != rows.device:
-        _refuse(f"out: expected {n} rows of {dim} columns on {rows.device}")
+        out = Q8Rows.empty(n, dim, dev)
+    elif len(out) != n or out.dim != dim or out.codes.device != dev:
+        _refuse(f"out: expected {n} rows of {dim} columns on {dev}")
     api = _api()
-    api.check(api.fn.q8_quantize_dev(rows.data_ptr(), _DTYPES[rows.dtype], stride, C.byref(out._c), _stream(rows)))
+    api.check(api.fn.q8_quantize_dev(rows.data_ptr(), kind, stride, C.byref(out._c), _raw_stream(dev.index)))
     return out
 
 
@@ -136,9 +155,9 @@ def score_rows(queries, base, metric, out=None):
         _refuse(f"queries are on {queries.codes.device}, not on {dev}")
     if queries.dim != base.dim:
         raise VectorLengthMismatch(f"Vector length mismatch: expected {base.dim}, got {queries.dim}")
-    out, stride = _out(out, len(queries), len(base), dev)
+    out, stride = _out(out, queries._c.n, base._c.n, dev)
     api = _api()
-    api.check(api.fn.q8_score_dev(C.byref(queries._c), C.byref(base._c), _metric(metric), out.data_ptr(), stride, _stream(out)))
+    api.check(api.fn.q8_score_dev(C.byref(queries._c), C.byref(base._c), _metric(metric), out.data_ptr(), stride, _raw_stream(dev.index)))
     return out
 
 
@@ -155,12 +174,14 @@ def adjust_scores(scores, metric, *, pass_bits=None, boost=None, seen=None, seen
     how = ScoreAdjustC()
 
     def per_query(t, what, dtype, width):
-        if t.dim() == 1:
-            t = t.unsqueeze(0)
-        s = _check(t, what, dtype, 2, dev)
-        if t.shape[1] < width or t.shape[0] not in (1, nq):
+        if isinstance(t, torch.Tensor) and t.dim() == 1:
+            _check(t, what, dtype, 1, dev)
+            rows, s = 1, 0
+        else:
+            s, rows = _check(t, what, dtype, 2, dev), t.shape[0]
+        if t.shape[-1] < width or rows not in (1, nq):
             _refuse(f"{what}: expected 1 or {nq} rows of {width}")
-        return t.data_ptr(), s if t.shape[0] > 1 else 0
+        return t.data_ptr(), s if rows > 1 else 0
 
     if pass_bits is not None:
         how.pass_bits, how.pass_stride = per_query(pass_bits, "pass_bits", torch.int32, -(-n // 32))
@@ -187,5 +208,5 @@ def adjust_scores(scores, metric, *, pass_bits=None, boost=None, seen=None, seen
         setattr(how, what, t.data_ptr())
     out, out_stride = _out(out, nq, n, dev)
     api = _api()
-    api.check(api.fn.score_adjust_dev(scores.data_ptr(), stride, nq, n, metric, C.byref(how), out.data_ptr(), out_stride, _stream(scores)))
+    api.check(api.fn.score_adjust_dev(scores.data_ptr(), stride, nq, n, metric, C.byref(how), out.data_ptr(), out_stride, _raw_stream(dev.index)))
     return out
