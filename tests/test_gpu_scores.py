@@ -201,6 +201,19 @@ def test_score_rows_lie_apart_and_what_is_between_stays(vdb, nq):
         assert bool((room[:, :at] == -5).all()) and bool((room[:, at + 333:] == -5).all())
 
 
+@pytest.mark.parametrize("nq,n", [(2, 9), (20, 40), (300, 12)])
+def test_rows_very_far_apart(vdb, nq, n):
+    """Rows 16 MiB and more apart: beyond what the offsets of the tiled kernel hold."""
+    step = (1 << 24) + 16
+    b = S.quantize_rows(gauss(n, 300, 2).cuda())
+    room = torch.empty(n * step, dtype=torch.uint8, device="cuda").as_strided((n, 304), (step, 1))
+    room.copy_(b.codes)
+    far = S.Q8Rows(room, b.scales, b.norms2, 300)
+    q = S.quantize_rows(gauss(nq, 300, 1).cuda())
+    check_scores(S.score_rows(q, far, M.Cosine), held(q), held(b), M.Cosine, 300)
+    check_scores(S.score_rows(far, q, M.Euclidean), held(b), held(q), M.Euclidean, 300)
+
+
 @pytest.mark.parametrize("nq,n,dim", [(5, 40, 256), (40, 300, 256), (300, 300, 384)])
 def test_scales_far_apart(vdb, nq, n, dim):
     """Blocks from 2^-60 to 2^60 whose products meet in the middle."""

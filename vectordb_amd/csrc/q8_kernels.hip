@@ -251,7 +251,7 @@ struct TileOrder {
 
 template <int BM, int BN, int WM, int WN, int S>
 __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN))
-gemm_kernel(Q8View q, Q8View b, int metric, float* __restrict__ out, size_t out_stride, TileOrder order) {
+gemm_kernel(Q8View q, Q8View b, int metric, float* __restrict__ out, size_t out_stride, TileOrder order, bool streaming) {
     constexpr int WAVES = (BM / WM) * (BN / WN), ROWS = BM + BN;
     constexpr int KS = 64, CH = KS / 16, RPI = 64 / CH;        // columns per step, chunks per row, rows per load instruction of a wavefront
     constexpr int LOADS = ROWS / (RPI * WAVES);                // load instructions per wavefront and step
@@ -381,7 +381,8 @@ gemm_kernel(Q8View q, Q8View b, int metric, float* __restrict__ out, size_t out_
                 Run v;
 #pragma unroll
                 for (int i = 0; i < MT; ++i) v[i] = finish(acc[i][e / 16][e % 16 + k], nq[k], nb[i], METRIC);
-                if (whole) __builtin_nontemporal_store(v, reinterpret_cast<UnalignedRun*>(o));
+                if (whole && streaming) __builtin_nontemporal_store(v, reinterpret_cast<UnalignedRun*>(o));
+                else if (whole) *reinterpret_cast<UnalignedRun*>(o) = v;
                 else
 #pragma unroll
                     for (int i = 0; i < MT; ++i) if (row + i < b.n) o[i] = v[i];
@@ -445,6 +446,64 @@ gemm_kernel(Q8View q, Q8View b, int metric, float* __restrict__ out, size_t out_
         if (t >= end) break;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");           // nothing lands in LDS behind the workgroup's end
+}
+
+// Too few tiles for the kernel above: a workgroup scores 32 rows against 32 queries, its four wavefronts take a quarter of the columns
+// each, straight from memory to registers with the next block on its way, and add up in LDS, in one order.
+// It takes rows of any stride.
+__global__ void __launch_bounds__(256) narrow_kernel(Q8View q, Q8View b, int metric, float* __restrict__ out, size_t out_stride, uint32_t row_tiles, uint64_t tiles) {
+    __shared__ float part[4][16][64];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), r = lane & 31, g = lane >> 5;
+    for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+        const uint32_t row0 = (uint32_t)(t % row_tiles) * 32, q0 = (uint32_t)(t / row_tiles) * 32;
+        const uint32_t nb = b.blocks(), width = b.width(), lo = nb * wave / 4, hi = nb * (wave + 1) / 4;
+        const size_t row = row0 + min(r, b.n - 1 - row0), qu = q0 + min(r, q.n - 1 - q0);      // those behind the last repeat it and are not stored
+        const uint8_t* xc = b.codes + row * b.cs; const uint8_t* xs = b.scales + row * b.ss;
+        const uint8_t* yc = q.codes + qu * q.cs; const uint8_t* ys = q.scales + qu * q.ss;
+        floatx16 acc = {};
+        struct Block { uint4 x[4], y[4]; uint32_t xs, ys; };
+        auto load = [&](Block& to, uint32_t k) {
+            to.xs = xs[k]; to.ys = ys[k];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                const uint32_t at = k * Q8_BLOCK + 32 * h + 16 * g;
+                to.x[h] = load16(xc, at, width); to.y[h] = load16(yc, at, width);
+            }
+        };
+        auto multiply = [&](const Block& v) {
+            const float xf = scale_of(v.xs), yf = scale_of(v.ys);
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen(v.y[h].x, v.y[h].y, yf), widen(v.x[h].x, v.x[h].y, xf), acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen(v.y[h].z, v.y[h].w, yf), widen(v.x[h].z, v.x[h].w, xf), acc, 0, 0, 0);
+            }
+        };
+        Block u, v;
+        if (lo < hi) load(u, lo);
+        for (uint32_t k = lo; k < hi; k += 2) {
+            load(v, min(k + 1, hi - 1));
+            multiply(u);
+            if (k + 1 >= hi) break;
+            load(u, min(k + 2, hi - 1));
+            multiply(v);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) part[wave][e][lane] = acc[e];
+        __syncthreads();
+        // register 4 wave + e: row r of query 8 wave + 4 g + e
+        const uint64_t i = (uint64_t)row0 + r;
+        const float norm = norm_of(b.norms2, row, metric);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint64_t at = (uint64_t)q0 + 8 * wave + 4 * g + e;
+            if (at >= q.n || i >= b.n) continue;
+            float dot = part[0][4 * wave + e][lane];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) dot += part[w][4 * wave + e][lane];
+            out[at * out_stride + i] = finish(dot, norm_of(q.norms2, at, metric), norm, metric);
+        }
+        __syncthreads();                                       // the parts are read
+    }
 }
 
 // Up to 16 queries: bound by the pass over the rows, which go from memory to registers.  The queries' codes lie in LDS, 16-byte chunk
@@ -552,35 +611,6 @@ __global__ void __launch_bounds__(256) stream_kernel(Q8View q, Q8View b, int met
     }
 }
 
-// A wavefront scores 16 rows against 16 queries.
-__global__ void __launch_bounds__(256) score_kernel(Q8View q, Q8View b, int metric, float* __restrict__ out, size_t out_stride, uint32_t row_tiles, uint64_t tiles) {
-    const uint32_t lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const uint32_t nb = b.blocks(), width = b.width();
-    for (uint64_t t = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64; t < tiles; t += (uint64_t)gridDim.x * 4) {
-        const uint32_t row0 = (uint32_t)(t % row_tiles) * 16, q0 = (uint32_t)(t / row_tiles) * 16;
-        const size_t row = min(row0 + r, b.n - 1), qu = min(q0 + r, q.n - 1);          // a tile's end repeats the last row; what it gives is not stored
-        const uint8_t* rc = b.codes + row * b.cs; const uint8_t* qc = q.codes + qu * q.cs;
-        const uint8_t* rs = b.scales + row * b.ss; const uint8_t* qs = q.scales + qu * q.ss;
-        floatx4 acc{0.f, 0.f, 0.f, 0.f};
-        for (uint32_t k = 0; k < nb; ++k) {
-            const float xs = scale_of(rs[k]), ys = scale_of(qs[k]);
-#pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-                const uint4 x = load16(rc, k * Q8_BLOCK + 64 * h + 16 * g, width), y = load16(qc, k * Q8_BLOCK + 64 * h + 16 * g, width);
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(x.x, x.y, xs), widen(y.x, y.y, ys), acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(x.z, x.w, xs), widen(y.z, y.w, ys), acc, 0, 0, 0);
-            }
-        }
-        if (q0 + r >= q.n) continue;
-        const float nq = norm_of(q.norms2, qu, metric);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t c = row0 + 4 * g + i;
-            if (c < b.n) out[(size_t)qu * out_stride + c] = finish(acc[i], nq, norm_of(b.norms2, c, metric), metric);
-        }
-    }
-}
-
 }  // namespace
 
 template <class T> static void launch_quantize(const T* rows, size_t stride, const vdb_q8_rows& out, hipStream_t s) {
@@ -619,20 +649,16 @@ static void launch_gemm(const Q8View& q, const Q8View& b, int metric, float* out
         return std::max(cus * std::max(per_cu, 1), 8);
     }();
     const uint32_t grid = (uint32_t)std::min<uint64_t>(((uint64_t)rt * qt + 7) / 8, resident / 8) * 8;
-    hipLaunchKernelGGL((gemm_kernel<BM, BN, WM, WN, S>), dim3(grid), dim3(THREADS), 0, s, q, b, metric, out, out_stride, TileOrder{rt, qt, std::min<uint32_t>(qt, 2048 / BN)});
+    // Scores that fill whole lines leave with the streaming hint (1000 x 1M x 64: 753 against 784 us); where score rows begin inside a line
+    // the caches have to join their ends (3860 x 12917 x 84: 52 against 82 us with the hint, 128 x 200001 x 128 37 against 47), which
+    // pays off from 128 queries on (77 x 300007 x 100: 44 against 40).
+    const bool streaming = (out_stride % 32 == 0 && (uintptr_t)out % 128 == 0) || q.n < 128;
+    hipLaunchKernelGGL((gemm_kernel<BM, BN, WM, WN, S>), dim3(grid), dim3(THREADS), 0, s, q, b, metric, out, out_stride, TileOrder{rt, qt, std::min<uint32_t>(qt, 2048 / BN)},
+                       streaming);
     VDB_HIP(hipGetLastError());
 }
 
 void launch_q8_score(const Q8View& q, const Q8View& b, int metric, float* out, size_t out_stride, hipStream_t s) {
-    if ((q.n > 16 || b.width() > 4096) && q.cs <= MAX_STRIDE && b.cs <= MAX_STRIDE) {
-        // The larger the tile, the fewer conversions and LDS reads per product (1000 x 1M x 960: 2.08 / 2.48 / 3.56 ms), but it has to be
-        // filled and there have to be enough of them: 77 x 300007 x 100 45.6 / 37.1 / 41.7 us, 64 x 1M x 960 452 / 306 / 292 us,
-        // 300 x 5000 x 768 27.2 / 17.8 / 12.0 us.
-        if (q.n > 128 && tiles_of(b.n, 256) * tiles_of(q.n, 256) >= 512) launch_gemm<256, 256, 128, 64, 4>(q, b, metric, out, out_stride, s);
-        else if (q.n > 64 && tiles_of(b.n, 256) * tiles_of(q.n, 128) >= 256) launch_gemm<256, 128, 64, 64, 4>(q, b, metric, out, out_stride, s);
-        else launch_gemm<128, 64, 64, 32, 4>(q, b, metric, out, out_stride, s);
-        return;
-    }
     if (q.n <= 16 && b.width() <= 4096) {                      // 64 KiB of LDS for the queries
         const uint32_t nb = b.blocks(), groups = (uint32_t)tiles_of(b.n, 16);
         const size_t lds = (size_t)nb * 2048 + (nb + 3) / 4 * 64;
@@ -644,11 +670,19 @@ void launch_q8_score(const Q8View& q, const Q8View& b, int metric, float* out, s
         VDB_HIP(hipGetLastError());
         return;
     }
-    const uint32_t row_tiles = (uint32_t)(((uint64_t)b.n + 15) / 16);
-    const uint64_t tiles = (((uint64_t)q.n + 15) / 16) * row_tiles;
-    const uint32_t blocks = (uint32_t)std::min<uint64_t>((tiles + 3) / 4, 1u << 20);
-    hipLaunchKernelGGL(score_kernel, dim3(blocks), dim3(256), 0, s, q, b, metric, out, out_stride, row_tiles, tiles);
-    VDB_HIP(hipGetLastError());
+    // The larger the tile, the fewer conversions and LDS reads per product (1000 x 1M x 960: 2.08 / 2.48 / 3.56 ms), but it has to be
+    // filled and there have to be enough of them: 77 x 300007 x 100 45.6 / 37.1 / 41.7 us, 64 x 1M x 960 452 / 306 / 292 us, 300 x 5000 x 768
+    // 27.2 / 17.8 / 12.0 us.  Kernel times in tiles of 128 x 64 and of 32 x 32 with split columns: 64 x 8000 x 768 (63 tiles) 11.1 and 8.6 us,
+    // 228 x 1130 x 3090 (36) 30.9 and 12.6, 64 x 16000 x 768 (125) 11.6 and 13.6.
+    const bool strides = q.cs <= MAX_STRIDE && b.cs <= MAX_STRIDE;
+    if (!strides || tiles_of(b.n, 128) * tiles_of(q.n, 64) < 96) {
+        const uint32_t rt = (uint32_t)tiles_of(b.n, 32);
+        const uint64_t tiles = rt * tiles_of(q.n, 32);
+        hipLaunchKernelGGL(narrow_kernel, dim3((uint32_t)std::min<uint64_t>(tiles, 1u << 20)), dim3(256), 0, s, q, b, metric, out, out_stride, rt, tiles);
+        VDB_HIP(hipGetLastError());
+    } else if (q.n > 128 && tiles_of(b.n, 256) * tiles_of(q.n, 256) >= 512) launch_gemm<256, 256, 128, 64, 4>(q, b, metric, out, out_stride, s);
+    else if (q.n > 64 && tiles_of(b.n, 256) * tiles_of(q.n, 128) >= 256) launch_gemm<256, 128, 64, 64, 4>(q, b, metric, out, out_stride, s);
+    else launch_gemm<128, 64, 64, 32, 4>(q, b, metric, out, out_stride, s);
 }
 
 }  // namespace vdb
