@@ -9,6 +9,8 @@ namespace {
 // A workgroup takes a span of columns of one query, four consecutive columns per thread and piece.  The scores are on their way while
 // the span's columns of the query's list are counted in LDS (integer atomics: the same counts in any order); then every score is
 // written once.  Bound by HBM: 8 bytes per column, 4 more for boosts.  Rows need no more than the alignment of a float.
+// Workgroups are dealt to the eight dies in turn: all queries of a span go to one die, one behind the other, so that a bitmap or a row
+// of boosts that they share is read once (16 x 1000003 with both: 22.4 us, query by query 28.3).
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef floatx4 floatx4_u __attribute__((aligned(4)));
 
@@ -17,7 +19,9 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(AdjustArgs a, uint32_t 
     constexpr int PIECES = SPAN / (4 * THREADS);
     __shared__ uint4 count[SEEN ? SPAN / 4 : 1];
     for (uint64_t t = blockIdx.x; t < tasks; t += gridDim.x) {
-        const uint32_t q = (uint32_t)(t / spans), lo = (uint32_t)(t % spans) * SPAN, m = min((uint32_t)SPAN, a.n - lo);
+        const uint64_t span = t / (8ull * a.nq) * 8 + t % 8;
+        if (span >= spans) continue;                           // of the whole workgroup
+        const uint32_t q = (uint32_t)(t / 8 % a.nq), lo = (uint32_t)span * SPAN, m = min((uint32_t)SPAN, a.n - lo);
         const float* scores = a.scores + q * a.stride + lo;
         floatx4 g[PIECES];
 #pragma unroll
@@ -35,9 +39,12 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(AdjustArgs a, uint32_t 
             for (int p = 0; p < PIECES; ++p) count[p * THREADS + threadIdx.x] = uint4{0, 0, 0, 0};
             __syncthreads();
             const uint64_t end = min(a.how.seen_offsets[q + 1], (uint64_t)a.how.n_seen);
-            for (uint64_t i = a.how.seen_offsets[q] + threadIdx.x; i < end; i += THREADS) {
-                const uint32_t c = a.how.seen[i] - lo;         // columns before lo wrap far beyond m
-                if (c < m) atomicAdd(reinterpret_cast<uint32_t*>(count) + c, 1u);
+            for (uint64_t i = a.how.seen_offsets[q] + threadIdx.x; i < end; i += 4 * THREADS) {
+                uint32_t c[4];                                 // four loads on their way; columns before lo wrap far beyond m
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[e] = i + e * THREADS < end ? a.how.seen[i + e * THREADS] - lo : m;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) if (c[e] < m) atomicAdd(reinterpret_cast<uint32_t*>(count) + c[e], 1u);
             }
             if (a.how.repeat) repeat = a.how.repeat[q];
             if (a.how.frequency) frequency = a.how.frequency[q];
@@ -89,7 +96,7 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(AdjustArgs a, uint32_t 
 template <int SPAN, int THREADS>
 static void launch(const AdjustArgs& a, hipStream_t s) {
     const uint32_t spans = (uint32_t)(((uint64_t)a.n + SPAN - 1) / SPAN);
-    const uint64_t tasks = (uint64_t)spans * a.nq;
+    const uint64_t tasks = ((uint64_t)spans + 7) / 8 * 8 * a.nq;
     const dim3 grid((uint32_t)std::min<uint64_t>(tasks, 1u << 20));
     if (a.how.seen) hipLaunchKernelGGL((adjust_kernel<SPAN, THREADS, true>), grid, dim3(THREADS), 0, s, a, spans, tasks);
     else hipLaunchKernelGGL((adjust_kernel<SPAN, THREADS, false>), grid, dim3(THREADS), 0, s, a, spans, tasks);
@@ -97,10 +104,11 @@ static void launch(const AdjustArgs& a, hipStream_t s) {
 }
 
 void launch_score_adjust(const AdjustArgs& a, hipStream_t s) {
-    // Every span reads its query's whole list again: long spans while they fill the chip (64 x 128000, lists of 3000: 19.2 us, spans of
-    // 4096 20.7 .. 23.8; lists of 30000: 33.9 against 65.3 .. 84.7), short ones else.
+    // Every span reads its query's whole list again, so long lists want long spans while they fill the chip (64 x 128000, lists of 3000:
+    // 14.4 us, spans of 4096 16.9; of 30000: 29.3 and 60.6); short lists want many workgroups (16 x 1000003, lists of 300: spans of 4096
+    // 26.7 us, of 16384 31.8).
     if (!a.how.seen) launch<4096, 256>(a, s);
-    else if (((uint64_t)a.n + 16383) / 16384 * a.nq >= 256) launch<16384, 1024>(a, s);
+    else if (a.how.n_seen / a.nq >= 1024 && ((uint64_t)a.n + 16383) / 16384 * a.nq >= 256) launch<16384, 512>(a, s);
     else launch<4096, 512>(a, s);
 }
 
