@@ -5,7 +5,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 h = re.sub(r'/\*.*?\*/', '', open(os.path.join(ROOT, "include/vdbmi.h")).read(), flags=re.S)
 have = set(re.findall(r'fn (vdb_[a-z0-9_]+)', open(os.path.join(ROOT, "rust/vectordb-mi355x/src/ffi.rs")).read()))
 SCALAR = {"size_t": "usize", "uint64_t": "u64", "uint32_t": "u32", "uint8_t": "u8", "int64_t": "i64", "int32_t": "i32", "int": "c_int",
-          "float": "f32", "double": "c_double", "char": "c_char", "void": "c_void", "vdb_status": "c_int", "vdb_metric": "c_int",
+          "float": "f32", "double": "c_double", "char": "c_char", "void": "c_void", "vdb_status": "c_int", "vdb_metric": "c_int", "vdb_dtype": "c_int",
           "vdb_scalar_op": "c_int", "vdb_list_query_kind": "c_int", "vdb_value_kind": "c_int"}
 def ty(c):
     c = c.strip()

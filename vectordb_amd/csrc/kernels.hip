@@ -120,7 +120,7 @@ __device__ __forceinline__ void fold_lanes(float* a, int g) {
 
 // FAST scan.  G lanes share a row (CH float4 each), a wave step covers R rows per group = R * 64 / G rows, and the rows
 // of the next step are in flight while this one is scored against the QT queries of the block (read from LDS once per
-// R rows).  Sums run as packed pairs (v_pk_fma_f32) and are folded across the group by fold_lanes.
+// R rows).  Sums run as pairs of floats and are folded across the group by fold_lanes.
 template <int G, int CH, int R, int QT, int NB>
 __global__ void __launch_bounds__(256) scan_fast_kernel(const float* __restrict__ queries, uint32_t nq, const float* __restrict__ base,
                                                        uint32_t n, uint32_t dim, uint32_t stride, int metric, float* __restrict__ out) {

@@ -331,7 +331,7 @@ struct Searcher {
 
     // Scores cand[0 .. m) into craw[0 .. m) (both LDS) for the register-resident beam: Euclidean
     // scores stay squared (the beam orders by them and takes the root once, when it hands the
-    // list over), sums run on packed two-float FMAs.  Lanes beyond the last candidate repeat it,
+    // list over), sums run on two-float FMAs.  Lanes beyond the last candidate repeat it,
     // so no lane is masked off.  FULL: a row fills all G x CH chunks, the stride is a constant.
     template <bool FULL> __device__ __forceinline__ void score_rows(int m) {
         typedef float f2 __attribute__((ext_vector_type(2)));
