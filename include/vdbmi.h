@@ -142,10 +142,11 @@ vdb_status vdb_score_scan_dev(const float* d_queries, size_t nq, const float* d_
  * nearest, ties to even, and at most 240 where the scale is 2^120 (so that every value is finite in f32); infinities and NaN
  * become the NaN code.
  *
- * Everything below reads and writes device memory, enqueues on `stream` (NULL = the null stream) and returns without waiting;
+ * Everything below but vdb_q8_score_scan works on device memory, enqueues on `stream` (NULL = the null stream) and returns without waiting;
  * nothing is allocated, so the calls may be captured into a graph and may overlap on different streams.  The work runs on the
  * device that owns the buffers, which must be one; the calling thread's current device is left as it was.  Host memory that
- * the device cannot read, NULL pointers, impossible sizes and misaligned buffers are VDB_ERR_ARGUMENT and nothing is launched;
+ * the device cannot read, NULL pointers, impossible sizes, misaligned buffers and outputs whose address range (first to last byte)
+ * meets another buffer's are VDB_ERR_ARGUMENT and nothing is launched;
  * zero rows or queries are VDB_OK and nothing is launched. */
 
 /* Element types of the rows handed to vdb_q8_quantize_dev. */
@@ -171,7 +172,7 @@ vdb_status vdb_q8_strides(size_t dim, size_t* code_stride, size_t* scale_stride)
 vdb_status vdb_q8_quantize_dev(const void* d_rows, vdb_dtype dtype, size_t stride, const vdb_q8_rows* out, void* stream);
 /* d_out[q * out_stride + i] = score of queries row q and base row i over the held values (score(), metric.rs:4-35): dot;
  * 1 - dot / (|q||i| + 1e-10); sqrt(max(0, |q|^2 + |i|^2 - 2 dot)) - the last one loses the digits that |q|^2 + |i|^2 and
- * 2 dot share.  Products are exact, sums are held in 32 bits.  out_stride >= base->n; d_out must not overlap the rows. */
+ * 2 dot share.  Products are exact, sums are held in 32 bits; sums below 2^-126 may count as zero.  out_stride >= base->n; d_out must not overlap the rows. */
 vdb_status vdb_q8_score_dev(const vdb_q8_rows* queries, const vdb_q8_rows* base, vdb_metric metric, float* d_out, size_t out_stride, void* stream);
 /* vdb_score_scan over 8-bit rows: host buffers in f32, quantised and scored on `device`, out[q * n + i]. */
 vdb_status vdb_q8_score_scan(const float* queries, size_t nq, const float* base, size_t n, size_t dim, vdb_metric metric, int device, float* out);

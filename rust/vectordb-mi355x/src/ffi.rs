@@ -15,6 +15,20 @@ use std::os::raw::{c_char, c_double, c_int, c_void};
 #[repr(C)] #[derive(Clone, Copy, Default)]
 pub struct vdb_scored_point { pub id: u64, pub raw_score: f32, pub sort_key: f32 }
 
+/// Rows held in 8 bits (device memory): e4m3 codes, one power-of-two scale per block of 128 columns, squared norms.
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct vdb_q8_rows { pub codes: *mut u8, pub scales: *mut u8, pub norms2: *mut f32, pub n: usize, pub dim: usize, pub code_stride: usize, pub scale_stride: usize }
+pub const VDB_F32: c_int = 0;
+pub const VDB_F16: c_int = 1;
+pub const VDB_BF16: c_int = 2;
+/// What is laid over dense score rows; null members are left out.
+#[repr(C)] #[derive(Clone, Copy)]
+pub struct vdb_score_adjust {
+    pub pass: *const u32, pub pass_stride: usize, pub boost: *const f32, pub boost_stride: usize,
+    pub seen: *const u32, pub seen_offsets: *const u64, pub n_seen: usize,
+    pub repeat: *const f32, pub frequency: *const f32, pub presence: *const f32,
+}
+
 /// per-query work counters (vdbmi.h: vdb_query_stats)
 #[repr(C)] #[derive(Clone, Copy, Default)]
 pub struct vdb_query_stats { pub rows_scored: u32, pub expanded: u32, pub adj_entries: u32, pub flags: u32 }
@@ -104,6 +118,11 @@ extern "C" {
     pub fn vdb_device_count() -> c_int;
     pub fn vdb_score_scan(queries: *const f32, nq: usize, base: *const f32, n: usize, dim: usize, metric: c_int, arith: c_int, device: c_int, out: *mut f32) -> c_int;
     pub fn vdb_score_scan_dev(d_queries: *const f32, nq: usize, d_base: *const f32, n: usize, dim: usize, stride: usize, metric: c_int, arith: c_int, d_out: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn vdb_q8_strides(dim: usize, code_stride: *mut usize, scale_stride: *mut usize) -> c_int;
+    pub fn vdb_q8_quantize_dev(d_rows: *const c_void, dtype: c_int, stride: usize, out: *const vdb_q8_rows, stream: *mut c_void) -> c_int;
+    pub fn vdb_q8_score_dev(queries: *const vdb_q8_rows, base: *const vdb_q8_rows, metric: c_int, d_out: *mut f32, out_stride: usize, stream: *mut c_void) -> c_int;
+    pub fn vdb_q8_score_scan(queries: *const f32, nq: usize, base: *const f32, n: usize, dim: usize, metric: c_int, device: c_int, out: *mut f32) -> c_int;
+    pub fn vdb_score_adjust_dev(d_scores: *const f32, stride: usize, nq: usize, n: usize, metric: c_int, how: *const vdb_score_adjust, d_out: *mut f32, out_stride: usize, stream: *mut c_void) -> c_int;
     pub fn vdb_value_type(v: *const vdb_value) -> c_int;
     pub fn vdb_value_equals(a: *const vdb_value, b: *const vdb_value) -> c_int;
     pub fn vdb_value_compare_scalar(a: *const vdb_value, op: c_int, b: *const vdb_value, is_some: *mut c_int, out: *mut c_int) -> c_int;

@@ -224,6 +224,20 @@ def test_scales_far_apart(vdb, nq, n, dim):
     check_scores(S.score_rows(q, b, M.Dot), held(q), held(b), M.Dot, dim)
 
 
+@pytest.mark.parametrize("nq,n", [(3, 100), (40, 200), (200, 12000)])
+@pytest.mark.parametrize("q_scale", [1e-20, 1e-7, 1e-3, 1.0, 1e9, 9e17])
+@pytest.mark.parametrize("b_scale", [1e-20, 1e-4, 1.0, 9e17])
+def test_small_and_large_rows(vdb, nq, n, q_scale, b_scale):
+    """The 1e-10 beside small norms, and norms whose product is beyond what a reciprocal holds."""
+    x, y = gauss(nq, 200, 1, 0.1), gauss(n, 200, 2, 0.1)
+    x, y = x / x.norm(dim=1, keepdim=True) * 14, y / y.norm(dim=1, keepdim=True) * 14
+    y[::3] *= 0.7
+    q, b = S.quantize_rows((x * q_scale).cuda()), S.quantize_rows((y * b_scale).cuda())
+    check_scores(S.score_rows(q, b, M.Cosine), held(q), held(b), M.Cosine, 200)
+    if min(q_scale, b_scale) >= 1e-7 and max(q_scale, b_scale) <= 1e9:              # products of smaller ones are subnormal; (14 * 9e17)^2 twice is beyond f32
+        check_scores(S.score_rows(q, b, M.Euclidean), held(q), held(b), M.Euclidean, 200)
+
+
 @pytest.mark.parametrize("nq,n", [(2, 30), (40, 40), (300, 300)])
 def test_nonfinite_rows_score_nan_and_no_others(vdb, nq, n):
     x, y = gauss(nq, 200, 1), gauss(n, 200, 2)
@@ -234,6 +248,21 @@ def test_nonfinite_rows_score_nan_and_no_others(vdb, nq, n):
         bad = torch.zeros(nq, n, dtype=torch.bool)
         bad[1] = True; bad[:, 3] = True; bad[:, n - 1] = True
         assert torch.equal(torch.isnan(s), bad)
+
+
+@pytest.mark.parametrize("nq,n", [(1, 50), (9, 3000), (20, 70), (70, 20000), (300, 30000)])
+def test_bytes_behind_a_row_do_not_matter(vdb, nq, n):
+    """NaN codes behind the row's 16-byte pieces, any scale behind its last block."""
+    dim = 150
+    q, b = S.quantize_rows(gauss(nq, dim, 1).cuda()), S.quantize_rows(gauss(n, dim, 2).cuda())
+    want = S.score_rows(q, b, M.Dot)
+
+    def wide(r):
+        w = S.Q8Rows(torch.full((len(r), 256), 0x7F, dtype=torch.uint8, device="cuda"), torch.full((len(r), 8), 255, dtype=torch.uint8, device="cuda"), None, dim)
+        w.codes[:, :160] = r.codes
+        w.scales[:, :2] = r.scales[:, :2]
+        return w
+    assert torch.equal(S.score_rows(wide(q), wide(b), M.Dot), want)
 
 
 def test_a_scale_of_255_is_nan(vdb):
@@ -346,7 +375,7 @@ def check_adjusted(got, want, mag):
     assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isinf(got), np.isinf(want))
     fin = np.isfinite(want)
     assert np.array_equal(np.sign(got[np.isinf(want)]), np.sign(want[np.isinf(want)]))
-    assert np.all(np.abs(got - want)[fin] <= (4 * U * mag)[fin])
+    assert np.all(np.abs(got[fin] - want[fin]) <= 4 * U * mag[fin])
 
 
 ADJUST = [(1, 1), (1, 31), (2, 32), (3, 33), (5, 100), (1, 10000), (4, 4095), (4, 4096), (4, 4097), (7, 8191), (2, 65537), (300, 129), (1, 300001)]

@@ -189,14 +189,25 @@ __device__ inline bf16x8 widen(uint32_t lo, uint32_t hi, float scale) {         
 }
 
 // Roots and reciprocals are the hardware's (one step off at most): the scores are FAST arithmetic.
-__device__ inline float root(float x) { return __builtin_amdgcn_sqrtf(x); }
+__device__ inline float root(float x) {                        // the instruction takes subnormals for zero
+    const bool tiny = x < 0x1p-96f;
+    const float y = __builtin_amdgcn_sqrtf(tiny ? x * 0x1p64f : x);
+    return tiny ? y * 0x1p-32f : y;
+}
+__device__ inline float inverse(float x) { return __builtin_amdgcn_rcpf(x); }
 // What a row's (query's) squared norm is used as.
 __device__ inline float norm_of(const float* norms2, size_t i, int metric) {
     return metric == VDB_DOT ? 0.f : metric == VDB_COSINE ? root(norms2[i]) : norms2[i];
 }
 __device__ inline float finish(float dot, float nq, float nb, int metric) {
     if (metric == VDB_DOT) return dot;
-    if (metric == VDB_COSINE) return __builtin_fmaf(-dot, __builtin_amdgcn_rcpf(__builtin_fmaf(nq, nb, 1e-10f)), 1.0f);
+    if (metric == VDB_COSINE) {
+        // The reciprocal of a product beyond 2^126 is too small for the instruction (and 1e-10 vanishes long before): one factor at a time.
+        const float both = nq * nb;
+        const bool far = both > 0x1p60f;
+        const float part = dot * inverse(far ? nq : both + 1e-10f);
+        return 1.0f - (far ? part * inverse(nb) : part);
+    }
     const float d = __builtin_fmaf(-2.f, dot, nq + nb);
     return root(d < 0.f ? 0.f : d);                            // NaN stays
 }
@@ -368,25 +379,42 @@ gemm_kernel(Q8View q, Q8View b, int metric, float* __restrict__ out, size_t out_
         for (int i = 0; i < MT; ++i) nb[i] = norm_of(b.norms2, min(row + i, (uint64_t)b.n - 1), METRIC);
         float* lane_base = out + ((size_t)q0 + 4 * g) * out_stride + row;
         const uint32_t left = q.n - 1 - q0;                    // the last query's place
+        // Lane l holds the norm of query l of the tile; a register's two queries are read from there.
+        static_assert(WN <= 64, "a lane per query");
+        const float lane_nq = norm_of(q.norms2, (size_t)q0 + min(lane % WN, left), METRIC);
+        float least = lane_nq;
 #pragma unroll
-        for (int e = 0; e < 16 * NT; e += 4) {                 // four queries at a time
-            float nq[4];
+        for (int i = 0; i < MT; ++i) least = min(least, nb[i]);
+        // Norms of 2^-4 and more: 1e-10 is less than half a step of their products, and the reciprocals may be taken apart.  Squared norms of
+        // 2^-60 and more: their sum less twice the product is zero or a multiple of 2^-84, so no subnormal meets the root.
+        const bool plain = METRIC != VDB_DOT && __all(least >= (METRIC == VDB_COSINE ? 0.0625f : 0x1p-60f));
+        const bool apart = METRIC == VDB_COSINE && plain;
+        const uint32_t lane_value = __float_as_uint(apart ? inverse(lane_nq) : lane_nq);
+        if (apart)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) nq[k] = norm_of(q.norms2, (size_t)q0 + min(2 * e + 4 * g + k, left), METRIC);
+            for (int i = 0; i < MT; ++i) nb[i] = inverse(nb[i]);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t at = 2 * e + k;
-                if (at + 4 * g > left) continue;
-                float* o = lane_base + (size_t)at * out_stride;
-                Run v;
+        for (int e = 0; e < 16 * NT; ++e) {
+            const uint32_t at = e / 4 * 8 + e % 4;             // and at + 4 in the upper half of the lanes
+            const float low = __uint_as_float(__builtin_amdgcn_readlane(lane_value, at)), high = __uint_as_float(__builtin_amdgcn_readlane(lane_value, at + 4));
+            const float nq = g ? high : low;
+            if (at + 4 * g > left) continue;
+            float* o = lane_base + (size_t)at * out_stride;
+            Run v;
 #pragma unroll
-                for (int i = 0; i < MT; ++i) v[i] = finish(acc[i][e / 16][e % 16 + k], nq[k], nb[i], METRIC);
-                if (whole && streaming) __builtin_nontemporal_store(v, reinterpret_cast<UnalignedRun*>(o));
-                else if (whole) *reinterpret_cast<UnalignedRun*>(o) = v;
-                else
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) if (row + i < b.n) o[i] = v[i];
+            for (int i = 0; i < MT; ++i) {
+                const float dot = acc[i][e / 16][e % 16];
+                if (apart) v[i] = __builtin_fmaf(dot * nq, -nb[i], 1.f);
+                else if (METRIC == VDB_EUCLIDEAN && plain) {
+                    const float d = __builtin_fmaf(-2.f, dot, nq + nb[i]);
+                    v[i] = __builtin_amdgcn_sqrtf(d < 0.f ? 0.f : d);
+                } else v[i] = finish(dot, nq, nb[i], METRIC);
             }
+            if (whole && streaming) __builtin_nontemporal_store(v, reinterpret_cast<UnalignedRun*>(o));
+            else if (whole) *reinterpret_cast<UnalignedRun*>(o) = v;
+            else
+#pragma unroll
+                for (int i = 0; i < MT; ++i) if (row + i < b.n) o[i] = v[i];
         }
     };
     auto store = [&] {
