@@ -373,7 +373,6 @@ gemm_kernel(Q8View q, Q8View b, int metric, float* __restrict__ out, size_t out_
     auto store_as = [&](auto kind, uint32_t row0, uint32_t q0) {
         constexpr int METRIC = decltype(kind)::value;
         const uint64_t row = (uint64_t)row0 + MT * r;
-        const bool whole = (uint64_t)row0 + WM <= b.n;
         float nb[MT];
 #pragma unroll
         for (int i = 0; i < MT; ++i) nb[i] = norm_of(b.norms2, min(row + i, (uint64_t)b.n - 1), METRIC);
@@ -381,40 +380,55 @@ gemm_kernel(Q8View q, Q8View b, int metric, float* __restrict__ out, size_t out_
         const uint32_t left = q.n - 1 - q0;                    // the last query's place
         // Lane l holds the norm of query l of the tile; a register's two queries are read from there.
         static_assert(WN <= 64, "a lane per query");
-        const float lane_nq = norm_of(q.norms2, (size_t)q0 + min(lane % WN, left), METRIC);
-        float least = lane_nq;
+        float lane_nq = norm_of(q.norms2, (size_t)q0 + min(lane % WN, left), METRIC), least = lane_nq;
 #pragma unroll
         for (int i = 0; i < MT; ++i) least = min(least, nb[i]);
-        // Norms of 2^-4 and more: 1e-10 is less than half a step of their products, and the reciprocals may be taken apart.  Squared norms of
-        // 2^-60 and more: their sum less twice the product is zero or a multiple of 2^-84, so no subnormal meets the root.
-        const bool plain = METRIC != VDB_DOT && __all(least >= (METRIC == VDB_COSINE ? 0.0625f : 0x1p-60f));
-        const bool apart = METRIC == VDB_COSINE && plain;
-        const uint32_t lane_value = __float_as_uint(apart ? inverse(lane_nq) : lane_nq);
-        if (apart)
+        // `easy`: norms of 2^-4 and more: 1e-10 is less than half a step of their products, and the reciprocals may be taken apart;
+        // squared norms of 2^-60 and more: their sum less twice the product is zero or a multiple of 2^-84, so no subnormal meets the root.
+        enum { EDGE, WHOLE, STREAMING };                       // whole: every row and query of the tile is there
+        auto put = [&](auto how, auto easy) {
+            constexpr int HOW = decltype(how)::value;
+            constexpr bool EASY = decltype(easy)::value;
+            float* o = lane_base;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) nb[i] = inverse(nb[i]);
+            for (int e = 0; e < 16 * NT; ++e) {
+                const uint32_t at = e / 4 * 8 + e % 4;         // and at + 4 in the upper half of the lanes
+                if (e) o += (e % 4 ? 1 : 5) * out_stride;
+                if (HOW == EDGE && at + 4 * g > left) continue;
+                float nq = 0.f;
+                if (METRIC != VDB_DOT) {
+                    const float low = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lane_nq), at)), high = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lane_nq), at + 4));
+                    nq = g ? high : low;
+                }
+                Run v;
 #pragma unroll
-        for (int e = 0; e < 16 * NT; ++e) {
-            const uint32_t at = e / 4 * 8 + e % 4;             // and at + 4 in the upper half of the lanes
-            const float low = __uint_as_float(__builtin_amdgcn_readlane(lane_value, at)), high = __uint_as_float(__builtin_amdgcn_readlane(lane_value, at + 4));
-            const float nq = g ? high : low;
-            if (at + 4 * g > left) continue;
-            float* o = lane_base + (size_t)at * out_stride;
-            Run v;
+                for (int i = 0; i < MT; ++i) {
+                    const float dot = acc[i][e / 16][e % 16];
+                    if (EASY && METRIC == VDB_COSINE) v[i] = __builtin_fmaf(dot * nq, -nb[i], 1.f);       // norms hold their reciprocals
+                    else if (EASY && METRIC == VDB_EUCLIDEAN) {
+                        const float d = __builtin_fmaf(-2.f, dot, nq + nb[i]);
+                        v[i] = __builtin_amdgcn_sqrtf(d < 0.f ? 0.f : d);
+                    } else v[i] = finish(dot, nq, nb[i], METRIC);
+                }
+                if (HOW == STREAMING) {
+                    asm volatile("" ::: );                     // or the compiler makes one store of this and the one below, without the hint
+                    __builtin_nontemporal_store(v, reinterpret_cast<UnalignedRun*>(o));
+                } else if (HOW == WHOLE) *reinterpret_cast<UnalignedRun*>(o) = v;
+                else
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const float dot = acc[i][e / 16][e % 16];
-                if (apart) v[i] = __builtin_fmaf(dot * nq, -nb[i], 1.f);
-                else if (METRIC == VDB_EUCLIDEAN && plain) {
-                    const float d = __builtin_fmaf(-2.f, dot, nq + nb[i]);
-                    v[i] = __builtin_amdgcn_sqrtf(d < 0.f ? 0.f : d);
-                } else v[i] = finish(dot, nq, nb[i], METRIC);
+                    for (int i = 0; i < MT; ++i) if (row + i < b.n) o[i] = v[i];
             }
-            if (whole && streaming) __builtin_nontemporal_store(v, reinterpret_cast<UnalignedRun*>(o));
-            else if (whole) *reinterpret_cast<UnalignedRun*>(o) = v;
-            else
+        };
+        const std::integral_constant<int, EDGE> edge; const std::integral_constant<int, WHOLE> whole; const std::integral_constant<int, STREAMING> stream;
+        if ((uint64_t)row0 + WM > b.n || left < WN - 1) put(edge, std::false_type{});
+        else if (METRIC != VDB_DOT && !__all(least >= (METRIC == VDB_COSINE ? 0.0625f : 0x1p-60f))) put(whole, std::false_type{});
+        else {
+            if (METRIC == VDB_COSINE) {
+                lane_nq = inverse(lane_nq);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) if (row + i < b.n) o[i] = v[i];
+                for (int i = 0; i < MT; ++i) nb[i] = inverse(nb[i]);
+            }
+            if (streaming) put(stream, std::true_type{}); else put(whole, std::true_type{});
         }
     };
     auto store = [&] {
@@ -677,10 +691,10 @@ static void launch_gemm(const Q8View& q, const Q8View& b, int metric, float* out
         return std::max(cus * std::max(per_cu, 1), 8);
     }();
     const uint32_t grid = (uint32_t)std::min<uint64_t>(((uint64_t)rt * qt + 7) / 8, resident / 8) * 8;
-    // Scores that fill whole lines leave with the streaming hint (1000 x 1M x 64: 753 against 784 us); where score rows begin inside a line
-    // the caches have to join their ends (3860 x 12917 x 84: 52 against 82 us with the hint, 128 x 200001 x 128 37 against 47), which
-    // pays off from 128 queries on (77 x 300007 x 100: 44 against 40).
-    const bool streaming = (out_stride % 32 == 0 && (uintptr_t)out % 128 == 0) || q.n < 128;
+    // Scores that the last-level cache (256 MB) cannot keep leave with the streaming hint (1000 x 1M x 64: 784 against 853 us, 8000 x 125000 x 960
+    // 1837 against 2327, 64 x 1M x 64 54 against 71; but 3860 x 12928 x 84, 200 MB, 49 against 42), unless score rows begin inside a sector of
+    // 32 bytes, whose parts have to be joined (1000 x 1000002 x 64: 1358 against 1210, 128 x 200001 x 128 42 against 26).
+    const bool streaming = 4.0 * q.n * b.n > 235e6 && out_stride % 8 == 0 && (uintptr_t)out % 32 == 0;
     hipLaunchKernelGGL((gemm_kernel<BM, BN, WM, WN, S>), dim3(grid), dim3(THREADS), 0, s, q, b, metric, out, out_stride, TileOrder{rt, qt, std::min<uint32_t>(qt, 2048 / BN)},
                        streaming);
     VDB_HIP(hipGetLastError());
