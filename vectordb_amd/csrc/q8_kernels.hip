@@ -712,18 +712,25 @@ void launch_q8_score(const Q8View& q, const Q8View& b, int metric, float* out, s
         VDB_HIP(hipGetLastError());
         return;
     }
-    // The larger the tile, the fewer conversions and LDS reads per product (1000 x 1M x 960: 2.08 / 2.48 / 3.56 ms), but it has to be
-    // filled and there have to be enough of them: 77 x 300007 x 100 45.6 / 37.1 / 41.7 us, 64 x 1M x 960 452 / 306 / 292 us, 300 x 5000 x 768
-    // 27.2 / 17.8 / 12.0 us.  Kernel times in tiles of 128 x 64 and of 32 x 32 with split columns: 64 x 8000 x 768 (63 tiles) 11.1 and 8.6 us,
-    // 228 x 1130 x 3090 (36) 30.9 and 12.6, 64 x 16000 x 768 (125) 11.6 and 13.6.
-    const bool strides = q.cs <= MAX_STRIDE && b.cs <= MAX_STRIDE;
-    if (!strides || tiles_of(b.n, 128) * tiles_of(q.n, 64) < 96) {
+    const uint64_t small = tiles_of(b.n, 128) * tiles_of(q.n, 64);
+    if (q.cs > MAX_STRIDE || b.cs > MAX_STRIDE || small < 96) {
+        // Kernel times in tiles of 128 x 64 and of 32 x 32 with split columns: 64 x 8000 x 768 (63 tiles) 11.1 and 8.6 us, 228 x 1130 x 3090
+        // (36) 30.9 and 12.6, 64 x 16000 x 768 (125) 11.6 and 13.6.
         const uint32_t rt = (uint32_t)tiles_of(b.n, 32);
         const uint64_t tiles = rt * tiles_of(q.n, 32);
         hipLaunchKernelGGL(narrow_kernel, dim3((uint32_t)std::min<uint64_t>(tiles, 1u << 20)), dim3(256), 0, s, q, b, metric, out, out_stride, rt, tiles);
         VDB_HIP(hipGetLastError());
-    } else if (q.n > 128 && tiles_of(b.n, 256) * tiles_of(q.n, 256) >= 512) launch_gemm<256, 256, 128, 64, 4>(q, b, metric, out, out_stride, s);
-    else if (q.n > 64 && tiles_of(b.n, 256) * tiles_of(q.n, 128) >= 256) launch_gemm<256, 128, 64, 64, 4>(q, b, metric, out, out_stride, s);
+        return;
+    }
+    // The larger the tile, the fewer conversions and LDS reads per product, but the chip works in rounds: it holds 256, 256 and 768 tiles
+    // of the three sizes, and a round of them takes 24, 15.5 and 13 us on rows of 768.  The least sum is taken.  In tiles of 256 x 256 /
+    // 256 x 128 / 128 x 64: 1000 x 1M x 960 2123 / 2592 / 3601 us, 300 x 40000 x 768 46.8 / 30.7 / 33.0, 128 x 20000 x 768 22.6 / 16.4 / 13.5,
+    // 4000 x 4000 x 768 31.5 / 33.1 / 39.3, 64 x 1M x 960 454 / 332 / 294.
+    auto rounds = [](uint64_t tiles, uint64_t held) { return (tiles + held - 1) / held; };
+    const uint64_t large = rounds(tiles_of(b.n, 256) * tiles_of(q.n, 256), 256) * 48, middle = rounds(tiles_of(b.n, 256) * tiles_of(q.n, 128), 256) * 31;
+    const uint64_t least = rounds(small, 768) * 26;
+    if (large <= middle && large <= least) launch_gemm<256, 256, 128, 64, 4>(q, b, metric, out, out_stride, s);
+    else if (middle <= least) launch_gemm<256, 128, 64, 64, 4>(q, b, metric, out, out_stride, s);
     else launch_gemm<128, 64, 64, 32, 4>(q, b, metric, out, out_stride, s);
 }
 
