@@ -181,7 +181,9 @@ def test_more_rows_than_a_grid_holds(vdb):
 
 SHAPES = [(1, 1, 1), (1, 15, 16), (2, 16, 17), (16, 17, 127), (17, 33, 128), (15, 64, 129), (3, 100, 100), (1, 1000, 960), (8, 1000, 960), (16, 999, 513),
           (31, 257, 260), (33, 513, 130), (64, 300, 640), (65, 255, 96), (100, 511, 300), (128, 256, 128), (129, 700, 1000), (200, 1000, 64), (256, 256, 512),
-          (257, 1025, 768), (300, 77, 2000), (513, 600, 144), (1000, 130, 960), (7, 50, 9000), (5, 40, 4096), (16, 40000, 640), (3, 40, 4097), (2, 33, 4100), (70, 90, 4100), (130, 260, 4224), (1, 70000, 32), (500, 5000, 112)]
+          (257, 1025, 768), (300, 77, 2000), (513, 600, 144), (1000, 130, 960), (7, 50, 9000), (5, 40, 4096), (16, 40000, 640), (3, 40, 4097), (2, 33, 4100), (70, 90, 4100), (130, 260, 4224), (1, 70000, 32), (500, 5000, 112),
+          # each tile size of the tiled kernel, whole tiles and ragged ones
+          (70, 20001, 300), (128, 12800, 64), (300, 60003, 70), (384, 51200, 128), (129, 50001, 200), (512, 25600, 192), (256, 65536, 16), (1000, 20003, 130)]
 
 
 @pytest.mark.parametrize("metric", list(M))
@@ -191,14 +193,16 @@ def test_scores_against_64_bits(vdb, metric, nq, n, dim):
     check_scores(S.score_rows(q, b, metric), held(q), held(b), metric, dim)
 
 
-@pytest.mark.parametrize("nq", [1, 20, 70, 300])
-def test_score_rows_lie_apart_and_what_is_between_stays(vdb, nq):
-    q, b = S.quantize_rows(gauss(nq, 200, 1).cuda()), S.quantize_rows(gauss(333, 200, 2).cuda())
-    for at, wide in ((0, 336), (1, 340), (3, 335)):
+@pytest.mark.parametrize("metric", list(M))
+@pytest.mark.parametrize("nq,n", [(1, 333), (20, 333), (70, 333), (300, 333), (100, 20011), (129, 50001), (300, 60003), (600, 120000)])
+def test_score_rows_lie_apart_and_what_is_between_stays(vdb, nq, n, metric):
+    q, b = S.quantize_rows(gauss(nq, 200, 1).cuda()), S.quantize_rows(gauss(n, 200, 2).cuda())
+    want = S.score_rows(q, b, metric)
+    for at, wide in ((0, n + 3), (1, n + 7), (3, n + 2), (8, n + 8 + -n % 8)):
         room = torch.full((nq, wide + 8), -5.0, device="cuda")
-        S.score_rows(q, b, M.Dot, out=room[:, at:at + 333])
-        assert torch.equal(room[:, at:at + 333], S.score_rows(q, b, M.Dot))
-        assert bool((room[:, :at] == -5).all()) and bool((room[:, at + 333:] == -5).all())
+        S.score_rows(q, b, metric, out=room[:, at:at + n])
+        assert torch.equal(room[:, at:at + n], want)
+        assert bool((room[:, :at] == -5).all()) and bool((room[:, at + n:] == -5).all())
 
 
 @pytest.mark.parametrize("nq,n", [(2, 9), (20, 40), (300, 12)])
@@ -214,7 +218,7 @@ def test_rows_very_far_apart(vdb, nq, n):
     check_scores(S.score_rows(far, q, M.Euclidean), held(b), held(q), M.Euclidean, 300)
 
 
-@pytest.mark.parametrize("nq,n,dim", [(5, 40, 256), (40, 300, 256), (300, 300, 384)])
+@pytest.mark.parametrize("nq,n,dim", [(5, 40, 256), (40, 300, 256), (300, 300, 384), (100, 20000, 256), (300, 30000, 384)])
 def test_scales_far_apart(vdb, nq, n, dim):
     """Blocks from 2^-60 to 2^60 whose products meet in the middle."""
     g = torch.Generator().manual_seed(4)
@@ -238,7 +242,7 @@ def test_small_and_large_rows(vdb, nq, n, q_scale, b_scale):
         check_scores(S.score_rows(q, b, M.Euclidean), held(q), held(b), M.Euclidean, 200)
 
 
-@pytest.mark.parametrize("nq,n", [(2, 30), (40, 40), (300, 300)])
+@pytest.mark.parametrize("nq,n", [(2, 30), (40, 40), (300, 300), (100, 20000), (300, 60000), (200, 50000)])
 def test_nonfinite_rows_score_nan_and_no_others(vdb, nq, n):
     x, y = gauss(nq, 200, 1), gauss(n, 200, 2)
     x[1, 150] = float("inf"); y[3, 7] = float("nan"); y[n - 1, 199] = float("-inf")
