@@ -712,26 +712,31 @@ void launch_q8_score(const Q8View& q, const Q8View& b, int metric, float* out, s
         VDB_HIP(hipGetLastError());
         return;
     }
-    const uint64_t small = tiles_of(b.n, 128) * tiles_of(q.n, 64);
-    if (q.cs > MAX_STRIDE || b.cs > MAX_STRIDE || small < 96) {
-        // Kernel times in tiles of 128 x 64 and of 32 x 32 with split columns: 64 x 8000 x 768 (63 tiles) 11.1 and 8.6 us, 228 x 1130 x 3090
-        // (36) 30.9 and 12.6, 64 x 16000 x 768 (125) 11.6 and 13.6.
-        const uint32_t rt = (uint32_t)tiles_of(b.n, 32);
-        const uint64_t tiles = rt * tiles_of(q.n, 32);
-        hipLaunchKernelGGL(narrow_kernel, dim3((uint32_t)std::min<uint64_t>(tiles, 1u << 20)), dim3(256), 0, s, q, b, metric, out, out_stride, rt, tiles);
+    const uint32_t rt = (uint32_t)tiles_of(b.n, 32);
+    const uint64_t narrow = rt * tiles_of(q.n, 32);
+    if (q.cs > MAX_STRIDE || b.cs > MAX_STRIDE || narrow <= 448) {
+        // Times in tiles of 32 x 32 with split columns and of 64 x 64: 256 x 1000 x 4096 (256 of them) 13.1 and 26.0 us, 600 x 600 x 960 (361)
+        // 6.7 and 8.6, but 100 x 4000 x 2048 (500) 14.4 and 14.5, 20 x 20000 x 768 (625) 11.6 and 9.7.
+        hipLaunchKernelGGL(narrow_kernel, dim3((uint32_t)std::min<uint64_t>(narrow, 1u << 20)), dim3(256), 0, s, q, b, metric, out, out_stride, rt, narrow);
         VDB_HIP(hipGetLastError());
         return;
     }
-    // The larger the tile, the fewer conversions and LDS reads per product, but the chip works in rounds: it holds 256, 256 and 768 tiles
-    // of the three sizes, and a round of them takes 24, 15.5 and 13 us on rows of 768.  The least sum is taken.  In tiles of 256 x 256 /
-    // 256 x 128 / 128 x 64: 1000 x 1M x 960 2123 / 2592 / 3601 us, 300 x 40000 x 768 46.8 / 30.7 / 33.0, 128 x 20000 x 768 22.6 / 16.4 / 13.5,
-    // 4000 x 4000 x 768 31.5 / 33.1 / 39.3, 64 x 1M x 960 454 / 332 / 294.
-    auto rounds = [](uint64_t tiles, uint64_t held) { return (tiles + held - 1) / held; };
-    const uint64_t large = rounds(tiles_of(b.n, 256) * tiles_of(q.n, 256), 256) * 48, middle = rounds(tiles_of(b.n, 256) * tiles_of(q.n, 128), 256) * 31;
-    const uint64_t least = rounds(small, 768) * 26;
-    if (large <= middle && large <= least) launch_gemm<256, 256, 128, 64, 4>(q, b, metric, out, out_stride, s);
-    else if (middle <= least) launch_gemm<256, 128, 64, 64, 4>(q, b, metric, out, out_stride, s);
-    else launch_gemm<128, 64, 64, 32, 4>(q, b, metric, out, out_stride, s);
+    // The larger the tile, the fewer conversions and LDS reads per product; the smaller, the more evenly tiles fall on the compute units
+    // and the sooner one is done.  With k tiles for the fullest of 256 compute units a size takes A + k w, in units of which a step of
+    // 64 columns scales both; A and w are fitted to 36 shapes and pick the fastest size or one at most 7 % behind it (16 % for 77 x 300007 x
+    // 100, whose last queries are half a tile).  In tiles of 256 x 256, 256 x 128, 128 x 128, 128 x 64 and 64 x 64, us:
+    //    678 x 729766 x  392   805   952  1088  1263  1423          64 x 1M     x 960   455  332  344  294  341
+    //   1093 x 121956 x   77   145   137   167   178   204          20 x 100000 x 384    25   18   17   14   13
+    //   1243 x   2485 x 3194    79    55    38    46    44         332 x 2060  x 1091    31   21   13   14   10
+    auto cost = [&](int bm, int bn, double once, double each) { return once + each * (double)((tiles_of(b.n, bm) * tiles_of(q.n, bn) + 255) / 256); };
+    const double costs[] = {cost(256, 256, 16, 42), cost(256, 128, 15, 21.5), cost(128, 128, 14, 11.2), cost(128, 64, 19, 8.4), cost(64, 64, 10.5, 5.5)};
+    switch (std::min_element(costs, costs + 5) - costs) {
+        case 0: return launch_gemm<256, 256, 128, 64, 4>(q, b, metric, out, out_stride, s);
+        case 1: return launch_gemm<256, 128, 64, 64, 4>(q, b, metric, out, out_stride, s);
+        case 2: return launch_gemm<128, 128, 64, 32, 4>(q, b, metric, out, out_stride, s);
+        case 3: return launch_gemm<128, 64, 64, 32, 4>(q, b, metric, out, out_stride, s);
+        default: return launch_gemm<64, 64, 32, 32, 4>(q, b, metric, out, out_stride, s);
+    }
 }
 
 }  // namespace vdb
