@@ -106,7 +106,10 @@ def gauss(n, dim, seed, spread=2.0):
 # ---------------------------------------------------------------- quantiser
 
 @pytest.mark.parametrize("kind", list(TYPES))
-@pytest.mark.parametrize("n,dim", [(1, 1), (3, 3), (9, 16), (5, 17), (33, 100), (8, 127), (7, 128), (17, 129), (2, 511), (3, 513), (6, 960), (2, 4100), (600, 300), (2049, 260), (2200, 129), (700, 90)])
+@pytest.mark.parametrize("n,dim", [(1, 1), (3, 3), (9, 16), (5, 17), (33, 100), (8, 127), (7, 128), (17, 129), (2, 511), (3, 513), (6, 960), (2, 4100), (600, 300), (2049, 260), (2200, 129), (700, 90),
+                                    # rows by groups of 4, 8, 16 and 32 lanes, by wavefronts and by workgroups, with and without a ragged end
+                                    (70, 4), (70, 5), (70, 7), (70, 8), (70, 12), (70, 15), (70, 31), (70, 32), (70, 33), (70, 63), (70, 64), (70, 65), (70, 112), (1, 2),
+                                    (2050, 511), (2050, 512), (2051, 513), (2060, 700), (2050, 960), (2051, 1667), (2049, 2048), (2049, 8400), (40, 8400)])
 def test_quantised_rows_equal_the_definition(vdb, kind, n, dim):
     x = gauss(n, dim, n * 1000 + dim).to(TYPES[kind])
     r = S.quantize_rows(x.cuda())
@@ -115,6 +118,33 @@ def test_quantised_rows_equal_the_definition(vdb, kind, n, dim):
     assert np.array_equal(r.scales.cpu().numpy(), scales)
     want = (vals * vals).sum(1)
     assert np.all(np.abs(r.norms2.cpu().numpy() - want) <= (8 * -(-dim // 128) + 20) * U * want)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n,dim", [(50, 3), (50, 20), (50, 40), (50, 70), (50, 130), (2100, 130), (2100, 600), (2100, 1030)])
+def test_special_values_in_every_kernel(vdb, kind, n, dim):
+    """Infinities, NaN, the largest values and signed zeros beside ordinary rows, wherever a row ends."""
+    t = TYPES[kind]
+    at = torch.arange(n)
+    x = gauss(n, dim, dim)
+    x[at % 11 == 10] *= 1e-6                                                        # f16: subnormals
+    x = x.to(t)
+    for i, v in enumerate((float("inf"), -float("inf"), float("nan"), torch.finfo(t).max, -torch.finfo(t).max, torch.finfo(t).smallest_normal, -0.0)):
+        rows = at[at % 11 == i]
+        x[rows, (rows * 7) % dim] = v
+        x[rows[::3], dim - 1] = v
+    x[at % 11 == 9] = 0
+    r = S.quantize_rows(x.cuda())
+    codes, scales, vals = plain_quantize(x.double().numpy())
+    assert np.array_equal(r.codes.cpu().numpy(), codes)
+    assert np.array_equal(r.scales.cpu().numpy(), scales)
+    with np.errstate(over="ignore", invalid="ignore"):
+        want = (vals * vals).sum(1)
+        got = r.norms2.cpu().numpy().astype(np.float64)
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        ok = ~np.isnan(want) & (want < 2.0 ** 127)
+        assert np.all(np.abs(got - want)[ok] <= (8 * -(-dim // 128) + 20) * U * want[ok] + 2.0 ** -140)
+        assert np.all(got[want > 2.0 ** 129] == np.inf)
 
 
 def test_special_values(vdb):

@@ -12,15 +12,19 @@ namespace {
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
 
 // ---------------------------------------------------------------- quantiser
 // Block of 128 columns, a = max |x| over its finite values: e = the smallest exponent from -100 on with a <= 448 * 2^e, code =
-// e4m3(x * 2^-e) (v_cvt_pk_fp8_f32: nearest, ties to even; x * 2^-e is never beyond 448).  The smallest code is 2^-9: with e >= -100
+// e4m3(x * 2^-e) (v_cvt_scalef32_pk_fp8: nearest, ties to even; x * 2^-e is never beyond 448).  The smallest code is 2^-9: with e >= -100
 // every value held is an ordinary bf16 and f32 number; at e = 120 codes end at 240, so that no value rounds up to 2^128.
-// A lane reads 16 bytes, so 32 (16) lanes hold a block: a load reads 512 (256) bytes in a row, a store writes a whole line of codes.
-// Such a group walks through a row, and the next block is on its way while one is converted.
-// Bound by HBM: 4 (2) bytes read, 1 + 1/128 written per column.  1M x 960 f32 903 us = 5.3 TB/s (without the streaming hint on the codes
-// 918, with it on the rows too 1020; 16 lanes of 32 bytes 1040; two rows side by side 1058), 300007 x 100 bf16 29 us.
+// A lane reads 16 bytes, so 32 (16) lanes hold a block.  A row belongs to a group of that many lanes or fewer, to a wavefront or to a
+// workgroup, by its length and the number of rows; the next 16 bytes are on their way while some are converted.
+// Bound by HBM: 4 (2) bytes read, 1 + 1/128 written per column.  1M x 960 f32 837 us = 5.75 TB/s, 300007 x 100 bf16 20 us = 4.8 TB/s (rows
+// of 100 columns leave lanes without work and lines in parts).  Few instructions count for short rows: with every value tested for
+// being finite and scaled by a multiplication of its own, 300007 x 128 bf16 took 27 us, 1M x 128 f16 75 instead of 64.
 
 constexpr size_t MAX_STRIDE = 1u << 24;     // of the rows that the tiled kernel takes: its offsets have 32 bits
 constexpr int MIN_EXP = -100, TOP_EXP = 120;
@@ -28,16 +32,29 @@ constexpr int MIN_EXP = -100, TOP_EXP = 120;
 template <int CTRL> __device__ inline uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true); }
 // Over the 16 lanes of a row: exchanges of neighbours, pairs, and two mirrors; over 32 across two rows.
 template <int LANES> __device__ inline uint32_t max_over(uint32_t v) {
-    v = max(v, dpp<0xB1>(v)); v = max(v, dpp<0x4E>(v)); v = max(v, dpp<0x141>(v)); v = max(v, dpp<0x140>(v));
+    v = max(v, dpp<0xB1>(v)); v = max(v, dpp<0x4E>(v));
+    if (LANES == 4) return v;
+    v = max(v, dpp<0x141>(v));
+    if (LANES == 8) return v;
+    v = max(v, dpp<0x140>(v));
     if (LANES == 16) return v;
     const auto w = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     return max(w[0], w[1]);
 }
 template <int LANES> __device__ inline float sum_over(float v) {
     v += __uint_as_float(dpp<0xB1>(__float_as_uint(v))); v += __uint_as_float(dpp<0x4E>(__float_as_uint(v)));
-    v += __uint_as_float(dpp<0x141>(__float_as_uint(v))); v += __uint_as_float(dpp<0x140>(__float_as_uint(v)));
+    if (LANES == 4) return v;
+    v += __uint_as_float(dpp<0x141>(__float_as_uint(v)));
+    if (LANES == 8) return v;
+    v += __uint_as_float(dpp<0x140>(__float_as_uint(v)));
     if (LANES == 16) return v;
     const auto w = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(w[0]) + __uint_as_float(w[1]);
+}
+
+__device__ inline float sum_of_wave(float v) {
+    v = sum_over<32>(v);
+    const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(w[0]) + __uint_as_float(w[1]);
 }
 
@@ -56,27 +73,86 @@ template <class T> __device__ inline Piece<T> load_piece(const T* row, uint32_t 
     return f;
 }
 
+// Of a piece that was read at dim - E the values from k on, zeros behind them.
+template <class T> __device__ inline Piece<T> shifted(const Piece<T>& in, uint32_t k, uint32_t dim) {
+    constexpr int E = 16 / sizeof(T);
+    const uint32_t at = dim - E, by = k > at ? min(k - at, (uint32_t)E) * (uint32_t)sizeof(T) : 0u;     // bytes
+    uint4 w = __builtin_bit_cast(uint4, in);
+    if (by & 16) w = uint4{0, 0, 0, 0};
+    if (by & 8) w = uint4{w.z, w.w, 0, 0};
+    if (by & 4) w = uint4{w.y, w.z, w.w, 0};
+    if (by & 2) w = uint4{w.x >> 16 | w.y << 16, w.y >> 16 | w.z << 16, w.z >> 16 | w.w << 16, w.w >> 16};
+    return __builtin_bit_cast(Piece<T>, w);
+}
+
+// The largest |x| as the bits of its f32: bits without the sign are ordered as the absolute values are, infinities and NaN above all.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ inline uint32_t largest(const Piece<float>& in) {
+    uint32_t a = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a = max(a, __float_as_uint(in.v[i]) & 0x7FFFFFFFu);
+    return a;
+}
+template <class T> __device__ inline uint32_t largest(const Piece<T>& in) {
+    u16x2 a{0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const T two[2] = {in.v[i], in.v[i + 1]};
+        a = __builtin_elementwise_max(a, __builtin_bit_cast(u16x2, two) & (unsigned short)0x7FFF);
+    }
+    return __float_as_uint(to_float(__builtin_bit_cast(T, max(a[0], a[1]))));
+}
+// Two values / scale as codes in half HI of w.
+template <bool HI> __device__ inline void code_pair(s16x2& w, const float* x, float scale) { w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, x[0], x[1], scale, HI); }
+template <bool HI> __device__ inline void code_pair(s16x2& w, const _Float16* x, float scale) { w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, f16x2{x[0], x[1]}, scale, HI); }
+template <bool HI> __device__ inline void code_pair(s16x2& w, const __bf16* x, float scale) { w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, bf16x2{x[0], x[1]}, scale, HI); }
+
 // What a group of lanes makes of a block: a lane's codes, the exponent, and the lane's share of the squared norm.
-template <class T> struct Coded {
-    static constexpr int E = 16 / sizeof(T), LANES = Q8_BLOCK / E;
+template <class T, int LANES> struct Coded {
+    static constexpr int E = 16 / sizeof(T);
     typedef uint32_t Codes __attribute__((ext_vector_type(E / 4)));
     Codes c;
     int e;
+    __device__ void scale_by(uint32_t a) {                     // a = m * 2^E with 1 <= m < 2, 448 = 1.75 * 2^8
+        e = (int)(a >> 23) - 127 - 8 + ((a & 0x7FFFFFu) > 0x600000u);
+        e = a == 0 ? 0 : max(e, MIN_EXP);
+    }
     __device__ Coded(const Piece<T>& in, float& norm) {
+        const uint32_t a = max_over<LANES>(largest(in));
+        scale_by(a);
+        // Infinities, NaN and the codes that end at 240 are asked for once per wavefront.
+        if (__builtin_expect(__any(a > 0x7F600000u), 0)) with_care(in);
+        else {
+            const float scale = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+            for (int h = 0; h < E / 4; ++h) {
+                s16x2 w{0, 0};
+                code_pair<false>(w, in.v + 4 * h, scale);
+                code_pair<true>(w, in.v + 4 * h + 2, scale);
+                c[h] = __builtin_bit_cast(uint32_t, w);
+            }
+        }
+        float sum = 0.f;                                       // of the squared codes
+#pragma unroll
+        for (int h = 0; h < E / 4; ++h) {
+            const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(c[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(c[h], true);
+            sum = __builtin_fmaf(lo[0], lo[0], sum); sum = __builtin_fmaf(lo[1], lo[1], sum);
+            sum = __builtin_fmaf(hi[0], hi[0], sum); sum = __builtin_fmaf(hi[1], hi[1], sum);
+        }
+        const float down = __uint_as_float((uint32_t)(127 + e) << 23);
+        norm = __builtin_fmaf(sum * down, down, norm);         // 2^240 is no f32: one factor at a time
+    }
+    __device__ void with_care(const Piece<T>& in) {
         float x[E];
-        uint32_t a = 0;                                        // ordered as the absolute values are
+        uint32_t a = 0;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             x[i] = to_float(in.v[i]);
             const uint32_t v = __float_as_uint(x[i]) & 0x7FFFFFFFu;
             a = max(a, v < 0x7F800000u ? v : 0u);
         }
-        a = max_over<LANES>(a);
-        // a = m * 2^E with 1 <= m < 2, 448 = 1.75 * 2^8
-        e = (int)(a >> 23) - 127 - 8 + ((a & 0x7FFFFFu) > 0x600000u);
-        e = a == 0 ? 0 : max(e, MIN_EXP);
-        const float up = __uint_as_float((uint32_t)(127 - e) << 23), down = __uint_as_float((uint32_t)(127 + e) << 23);
-        const float top = e == TOP_EXP ? 240.f : 448.f;
+        scale_by(max_over<LANES>(a));
+        const float up = __uint_as_float((uint32_t)(127 - e) << 23), top = e == TOP_EXP ? 240.f : 448.f;
 #pragma unroll
         for (int h = 0; h < E / 4; ++h) {
             float y[4];
@@ -86,18 +162,16 @@ template <class T> struct Coded {
             w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
 #pragma unroll
             for (int i = 0; i < 4; ++i) if ((__float_as_uint(x[4 * h + i]) & 0x7FFFFFFFu) >= 0x7F800000u) w = (w & ~(0xFFu << (8 * i))) | (0x7Fu << (8 * i));
-            const float v0 = __builtin_amdgcn_cvt_f32_fp8(w, 0) * down, v1 = __builtin_amdgcn_cvt_f32_fp8(w, 1) * down;
-            const float v2 = __builtin_amdgcn_cvt_f32_fp8(w, 2) * down, v3 = __builtin_amdgcn_cvt_f32_fp8(w, 3) * down;
-            norm = __builtin_fmaf(v0, v0, norm); norm = __builtin_fmaf(v1, v1, norm);
-            norm = __builtin_fmaf(v2, v2, norm); norm = __builtin_fmaf(v3, v3, norm);
             c[h] = w;
         }
     }
 };
 
-template <class T>
+template <class T> constexpr int BLOCK_LANES = Q8_BLOCK * sizeof(T) / 16;
+
+template <class T, int LANES, bool STREAMING>
 __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ rows, size_t stride, vdb_q8_rows out) {
-    constexpr int E = Coded<T>::E, LANES = Coded<T>::LANES, GROUPS = 256 / LANES;
+    constexpr int E = 16 / sizeof(T), GROUPS = 256 / LANES;
     const uint32_t lane = threadIdx.x % LANES, dim = (uint32_t)out.dim;
     const uint32_t nb = (dim + Q8_BLOCK - 1) / Q8_BLOCK, width = (dim + 15u) & ~15u;
     const size_t all = (size_t)gridDim.x * GROUPS;
@@ -105,8 +179,11 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ row
     if (r >= out.n) return;                                    // whole groups of lanes: the exchanges below stay within one
     uint32_t b = 0, next_b = 0, scales = 0;
     float norm = 0.f;
+    constexpr bool SHORT = LANES == 4;                         // rows that may be shorter than a load
     auto load = [&] {
-        const Piece<T> x = load_piece(rows + next_r * stride, next_b * Q8_BLOCK + lane * E, dim);
+        const uint32_t k = next_b * Q8_BLOCK + lane * E;
+        const T* row = rows + next_r * stride;
+        const Piece<T> x = SHORT ? load_piece(row, k, dim) : *reinterpret_cast<const Piece<T>*>(row + min(k, dim - E));
         if (++next_b < nb) return x;
         next_b = 0;
         if (out.n - next_r > all) next_r += all;               // behind the last row it comes again and is not used
@@ -114,11 +191,16 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ row
     };
     Piece<T> next = load();
     while (true) {
-        const Piece<T> x = next;
+        Piece<T> x = next;
         next = load();
-        const Coded<T> coded(x, norm);
+        if (!SHORT && (b + 1) * Q8_BLOCK > dim) x = shifted(x, b * Q8_BLOCK + lane * E, dim);
+        const Coded<T, LANES> coded(x, norm);
         const uint32_t k = b * Q8_BLOCK + lane * E;
-        if (k < width) __builtin_nontemporal_store(coded.c, reinterpret_cast<typename Coded<T>::Codes*>(out.codes + r * out.code_stride + k));
+        if (k < width) {
+            auto* to = reinterpret_cast<typename Coded<T, LANES>::Codes*>(out.codes + r * out.code_stride + k);
+            if (STREAMING) __builtin_nontemporal_store(coded.c, to);
+            else *to = coded.c;
+        }
         if (b % 4 == 0) scales = 0x7F7F7F7Fu;                  // blocks behind the last: 127
         scales = (scales & ~(0xFFu << (8 * (b % 4)))) | (uint32_t)(coded.e + 127) << (8 * (b % 4));
         const bool last = b + 1 == nb;
@@ -138,7 +220,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ row
 // Few rows: a workgroup per row, its blocks side by side.
 template <class T>
 __global__ void __launch_bounds__(256) quantize_row_kernel(const T* __restrict__ rows, size_t stride, vdb_q8_rows out) {
-    constexpr int E = Coded<T>::E, LANES = Coded<T>::LANES, GROUPS = 256 / LANES;
+    constexpr int E = 16 / sizeof(T), LANES = BLOCK_LANES<T>, GROUPS = 256 / LANES;
     __shared__ float part[GROUPS];
     const uint32_t lane = threadIdx.x % LANES, group = threadIdx.x / LANES, dim = (uint32_t)out.dim;
     const uint32_t nb = (dim + Q8_BLOCK - 1) / Q8_BLOCK, width = (dim + 15u) & ~15u;
@@ -150,8 +232,8 @@ __global__ void __launch_bounds__(256) quantize_row_kernel(const T* __restrict__
             continue;
         }
         const uint32_t k = b * Q8_BLOCK + lane * E;
-        const Coded<T> coded(load_piece(rows + r * stride, k, dim), norm);
-        if (k < width) *reinterpret_cast<typename Coded<T>::Codes*>(out.codes + r * out.code_stride + k) = coded.c;
+        const Coded<T, LANES> coded(load_piece(rows + r * stride, k, dim), norm);
+        if (k < width) *reinterpret_cast<typename Coded<T, LANES>::Codes*>(out.codes + r * out.code_stride + k) = coded.c;
         if (lane == 0) out.scales[r * out.scale_stride + b] = (uint8_t)(coded.e + 127);
     }
     norm = sum_over<LANES>(norm);
@@ -162,6 +244,46 @@ __global__ void __launch_bounds__(256) quantize_row_kernel(const T* __restrict__
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) norm += part[i];
     out.norms2[r] = norm;
+}
+
+// Long rows: a wavefront per row, 1024 bytes of it a step.
+template <class T, bool STREAMING>
+__global__ void __launch_bounds__(256) quantize_wave_kernel(const T* __restrict__ rows, size_t stride, vdb_q8_rows out) {
+    constexpr uint32_t E = 16 / sizeof(T), LANES = BLOCK_LANES<T>, BLOCKS = 64 / LANES, SPAN = 64 * E;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), dim = (uint32_t)out.dim;
+    const uint32_t nb = (dim + Q8_BLOCK - 1) / Q8_BLOCK, width = (dim + 15u) & ~15u, steps = (dim + SPAN - 1) / SPAN;
+    for (size_t r = (size_t)blockIdx.x * 4 + wave; r < out.n; r += (size_t)gridDim.x * 4) {
+        const T* row = rows + r * stride;
+        auto load = [&](uint32_t i) { return *reinterpret_cast<const Piece<T>*>(row + min(i * SPAN + lane * E, dim - E)); };
+        Piece<T> next = load(0);
+        float norm = 0.f;
+        int mine = 0;                                          // lane l: exponent of block l of 64
+        for (uint32_t i = 0; i < steps; ++i) {
+            const uint32_t k = i * SPAN + lane * E;
+            Piece<T> x = next;
+            next = load(min(i + 1, steps - 1));
+            if ((i + 1) * SPAN > dim) x = shifted(x, k, dim);  // blocks behind the last are zeros, with the scale that belongs there
+            const Coded<T, LANES> coded(x, norm);
+            if (k < width) {
+                auto* to = reinterpret_cast<typename Coded<T, LANES>::Codes*>(out.codes + r * out.code_stride + k);
+                if (STREAMING) __builtin_nontemporal_store(coded.c, to);
+                else *to = coded.c;
+            }
+            const uint32_t first = i * BLOCKS % 64;
+#pragma unroll
+            for (uint32_t g = 0; g < BLOCKS; ++g) {
+                const int e = __builtin_amdgcn_readlane(coded.e, g * LANES);
+                mine = lane == first + g ? e : mine;
+            }
+            if (first + BLOCKS < 64 && i + 1 < steps) continue;
+            const uint32_t b = i * BLOCKS / 64 * 64 + lane;
+            if (b < ((nb + 3) & ~3u)) out.scales[r * out.scale_stride + b] = (uint8_t)(mine + 127);
+            mine = 0;
+        }
+        if (!out.norms2) continue;
+        norm = sum_of_wave(norm);
+        if (lane == 0) out.norms2[r] = norm;
+    }
 }
 
 // ---------------------------------------------------------------- block-scaled product
@@ -175,7 +297,6 @@ __global__ void __launch_bounds__(256) quantize_row_kernel(const T* __restrict__
 // takes the 16 bytes at 16 g and at 64 + 16 g of row r, so that a load reads 64 consecutive bytes of each row.  The result's lane
 // (r, g) holds query r against rows 4 g .. 4 g + 3.
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 __device__ inline uint4 load16(const uint8_t* row, uint32_t k, uint32_t width) {
@@ -655,20 +776,43 @@ __global__ void __launch_bounds__(256) stream_kernel(Q8View q, Q8View b, int met
 
 }  // namespace
 
+template <class T, int LANES> static void launch_quantize_groups(const T* rows, size_t stride, const vdb_q8_rows& out, bool streaming, hipStream_t s) {
+    // A group per row while the grid allows, but rows of one block are over too soon for that (1M x 128: 142 against 130 us, 300007 x 100
+    // bf16: 31.5 against 29.1 on 8192 workgroups that walk on).
+    constexpr size_t per = 256 / LANES;
+    const uint32_t blocks = (uint32_t)std::min<size_t>((out.n + per - 1) / per, out.dim <= Q8_BLOCK ? 8192 : 1u << 18);
+    if (streaming) hipLaunchKernelGGL((quantize_kernel<T, LANES, true>), dim3(blocks), dim3(256), 0, s, rows, stride, out);
+    else hipLaunchKernelGGL((quantize_kernel<T, LANES, false>), dim3(blocks), dim3(256), 0, s, rows, stride, out);
+    VDB_HIP(hipGetLastError());
+}
+
 template <class T> static void launch_quantize(const T* rows, size_t stride, const vdb_q8_rows& out, hipStream_t s) {
-    // Kernel times for 1 / 500 / 2000 / 4000 rows of 960: 1.8 / 2.8 / 4.1 / 5.8 us a workgroup per row, 4.8 / 6.1 / 6.4 / 7.1 a group of lanes
-    // per row; 4000 x 256: 4.1 against 3.3.
+    // Times for 1 / 500 / 2000 / 8000 rows of 960: 2.2 / 2.8 / 3.6 / 8.0 us a workgroup per row, 2.9 / 3.5 / 3.7 / 6.6 a wavefront, 4.3 / 5.0
+    // / 5.3 / 7.9 a group of lanes; 4000 x 256: 4.1 a workgroup, 3.3 a group.
     if (out.n <= 2048 && out.dim > Q8_BLOCK) {
         hipLaunchKernelGGL(quantize_row_kernel<T>, dim3((uint32_t)out.n), dim3(256), 0, s, rows, stride, out);
         VDB_HIP(hipGetLastError());
         return;
     }
-    constexpr size_t per = 256 / Coded<T>::LANES;
-    // A group per row while the grid allows (1M x 960: 911 us; 8192 workgroups that walk on 993, 2048 1018), but rows of one block are over
-    // too soon for that (1M x 128: 142 against 130 us, 300007 x 100 bf16: 31.5 against 29.1).
-    const uint32_t blocks = (uint32_t)std::min<size_t>((out.n + per - 1) / per, out.dim <= Q8_BLOCK ? 8192 : 1u << 18);
-    hipLaunchKernelGGL(quantize_kernel<T>, dim3(blocks), dim3(256), 0, s, rows, stride, out);
-    VDB_HIP(hipGetLastError());
+    // Codes leave with the streaming hint unless rows begin inside half a line, whose parts have to be joined (400000 x 720 360 against 302 us,
+    // 744931 x 726 f16 460 against 397, but 1M x 128 132 against 137, 97895 x 1664 162 against 168).
+    const bool streaming = out.code_stride % 64 == 0 && (uintptr_t)out.codes % 64 == 0;
+    // A wavefront per row and a group of lanes per row: 1M x 960 837 and 959 us, 744931 x 726 f16 303 and 391, 1M x 512 417 and 432, f16 266 and
+    // 271, but 1M x 384 384 and 326, f16 254 and 194 (a million wavefronts take 250 us to start; fewer that walk on are slower on long
+    // rows: 65536 workgroups 860 us on 1M x 960, 2048 939).
+    if (out.dim >= 512) {
+        const uint32_t blocks = (uint32_t)std::min<size_t>((out.n + 3) / 4, 1u << 22);
+        if (streaming) hipLaunchKernelGGL((quantize_wave_kernel<T, true>), dim3(blocks), dim3(256), 0, s, rows, stride, out);
+        else hipLaunchKernelGGL((quantize_wave_kernel<T, false>), dim3(blocks), dim3(256), 0, s, rows, stride, out);
+        VDB_HIP(hipGetLastError());
+        return;
+    }
+    // Short rows take as many lanes as they fill, so that a wavefront holds more of them: 1M x 16 17 us (32 lanes a row: 111), 1M x 64 bf16 33 (80).
+    constexpr int E = 16 / sizeof(T);
+    if (out.dim <= 4 * E) return launch_quantize_groups<T, 4>(rows, stride, out, streaming, s);
+    if (out.dim <= 8 * E) return launch_quantize_groups<T, 8>(rows, stride, out, streaming, s);
+    if (out.dim <= 16 * E) return launch_quantize_groups<T, 16>(rows, stride, out, streaming, s);
+    launch_quantize_groups<T, BLOCK_LANES<T>>(rows, stride, out, streaming, s);
 }
 
 void launch_q8_quantize(const void* rows, int dtype, size_t stride, const vdb_q8_rows& out, hipStream_t s) {
