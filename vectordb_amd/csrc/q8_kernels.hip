@@ -670,13 +670,14 @@ __global__ void __launch_bounds__(256) narrow_kernel(Q8View q, Q8View b, int met
 }
 
 // Up to 16 queries: bound by the pass over the rows, which go from memory to registers.  The queries' codes lie in LDS, 16-byte chunk
-// by chunk.  A wavefront takes 16 rows at a time, a block of 128 columns a step, and has the next step's codes on their way while it
+// by chunk.  A wavefront takes 16 rows at a time, a block of 128 columns a step, and has DEPTH - 1 steps' codes on their way while it
 // multiplies one.  The queries are the left operand: a result register holds 16 rows of four queries.
-// Measured on 1 x 1M x 960: 171 us = 5.7 TB/s (8 queries 201 us); four blocks a step 166 us there and 113 instead of 109 us on 300000 x
-// 2048; 64 rows at a time 190 .. 212 us; with the streaming hint 190 us (the second half of a line is fetched again).
+// Measured on 1 x 1M x 960: 162 us = 6.0 TB/s, 8 queries 195 (with rows staged through LDS, 4 wavefronts and 16 rows of 256 columns a step,
+// 160 and 188, but 45 instead of 23 on 1M x 128); 64 rows at a time 190 .. 212 us; with the streaming hint 190 us (the second half of a line
+// is fetched again).
 // SPLIT: the four wavefronts of a workgroup take a quarter of the columns each of the same rows and add up in LDS, in one order.
-template <bool SPLIT>
-__global__ void __launch_bounds__(256) stream_kernel(Q8View q, Q8View b, int metric, float* __restrict__ out, size_t out_stride, uint32_t groups) {
+template <int METRIC, bool SPLIT, int DEPTH>
+__global__ void __launch_bounds__(256) stream_kernel(Q8View q, Q8View b, float* __restrict__ out, size_t out_stride, uint32_t groups) {
     extern __shared__ uint4 query[];                           // [8 chunks per block][16 queries], then the scales [4 blocks][16]
     __shared__ floatx4 part[3][SPLIT ? 64 : 1];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), r = lane & 15, g = lane >> 4;
@@ -687,24 +688,27 @@ __global__ void __launch_bounds__(256) stream_kernel(Q8View q, Q8View b, int met
     __syncthreads();
     float nq[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) nq[e] = norm_of(q.norms2, min(4 * g + e, q.n - 1), metric);
+    for (int e = 0; e < 4; ++e) nq[e] = norm_of(q.norms2, min(4 * g + e, q.n - 1), METRIC);
 
     const uint32_t first_group = SPLIT ? blockIdx.x : blockIdx.x * 4 + wave, stride = SPLIT ? gridDim.x : gridDim.x * 4;
     if (first_group >= groups) return;                         // SPLIT: of the whole workgroup
+    // Loads are on no condition, or the compiler could not tell how many are on their way and would wait for all of them: rows behind the
+    // last repeat it and are not stored, chunks behind a row's end repeat its last and meet zeros of the query.
     struct Step { uint4 v[2]; uint32_t scale; };
     const uint8_t* row; const uint8_t* row_scales;
-    auto go_to = [&](uint32_t group) {                         // rows behind the last repeat it; they are not stored
-        const size_t i = min((uint64_t)group * 16 + r, (uint64_t)b.n - 1);
-        row = b.codes + i * b.cs + 16 * g;
+    auto row_at = [&](uint32_t group) { return (size_t)min((uint64_t)group * 16 + r, (uint64_t)b.n - 1); };
+    auto go_to = [&](uint32_t group) {
+        const size_t i = row_at(group);
+        row = b.codes + i * b.cs;
         row_scales = b.scales + i * b.ss;
     };
     auto load = [&](Step& to, uint32_t k) {
         to.scale = row_scales[k];
-        const uint32_t at = k * Q8_BLOCK;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) to.v[h] = at + 64 * h + 16 * g < width ? *reinterpret_cast<const uint4*>(row + at + 64 * h) : uint4{0, 0, 0, 0};
+        for (int h = 0; h < 2; ++h) to.v[h] = *reinterpret_cast<const uint4*>(row + min(k * Q8_BLOCK + 64 * h + 16 * g, width - 16));
     };
     floatx4 acc{0.f, 0.f, 0.f, 0.f};
+    float norm;
     auto multiply = [&](const Step& x, uint32_t k) {
         const float qs = scale_of(query_scale[k / 4 * 16 + r] >> (8 * (k & 3)) & 255u), rs = scale_of(x.scale);
 #pragma unroll
@@ -717,24 +721,29 @@ __global__ void __launch_bounds__(256) stream_kernel(Q8View q, Q8View b, int met
     auto store = [&](uint32_t group) {
         const uint64_t i = (uint64_t)group * 16 + r;
         if (i >= b.n) return;
-        const float norm = norm_of(b.norms2, i, metric);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) if (4 * g + e < q.n) out[(size_t)(4 * g + e) * out_stride + i] = finish(acc[e], nq[e], norm, metric);
+        for (int e = 0; e < 4; ++e) if (4 * g + e < q.n) out[(size_t)(4 * g + e) * out_stride + i] = finish(acc[e], nq[e], METRIC == VDB_COSINE ? root(norm) : norm, METRIC);
     };
-    Step x, y;
+    auto load_norm = [&](uint32_t group) { norm = METRIC == VDB_DOT ? 0.f : b.norms2[row_at(group)]; };
+    Step step[DEPTH];
 
     if (SPLIT) {
         const uint32_t lo = nb * wave / 4, hi = nb * (wave + 1) / 4;
         for (uint32_t group = first_group; group < groups; group += stride) {
             go_to(group);
+            load_norm(group);
             acc = floatx4{0.f, 0.f, 0.f, 0.f};
-            if (lo < hi) load(x, lo);
-            for (uint32_t k = lo; k < hi; k += 2) {
-                load(y, min(k + 1, hi - 1));
-                multiply(x, k);
-                if (k + 1 >= hi) break;
-                load(x, min(k + 2, hi - 1));
-                multiply(y, k + 1);
+            if (lo < hi) {
+#pragma unroll
+                for (int i = 0; i < DEPTH - 1; ++i) load(step[i], min(lo + i, hi - 1));
+                for (uint32_t k = lo; k < hi; k += DEPTH) {
+#pragma unroll
+                    for (int i = 0; i < DEPTH; ++i) {
+                        if (k + i >= hi) break;
+                        load(step[(i + DEPTH - 1) % DEPTH], min(k + i + DEPTH - 1, hi - 1));
+                        multiply(step[i], k + i);
+                    }
+                }
             }
             __syncthreads();                                   // the parts of the last group are read
             if (wave) part[wave - 1][lane] = acc;
@@ -762,16 +771,19 @@ __global__ void __launch_bounds__(256) stream_kernel(Q8View q, Q8View b, int met
         acc = floatx4{0.f, 0.f, 0.f, 0.f};
         if (groups - group <= stride) return true;
         group += stride;
+        load_norm(group);
         return false;
     };
     go_to(group);
-    load_next(x);
-    while (true) {
-        load_next(y);
-        if (take(x)) return;
-        load_next(x);
-        if (take(y)) return;
-    }
+    load_norm(group);
+#pragma unroll
+    for (int i = 0; i < DEPTH - 1; ++i) load_next(step[i]);
+    while (true)
+#pragma unroll
+        for (int i = 0; i < DEPTH; ++i) {
+            load_next(step[(i + DEPTH - 1) % DEPTH]);
+            if (take(step[i])) return;
+        }
 }
 
 }  // namespace
@@ -848,11 +860,20 @@ void launch_q8_score(const Q8View& q, const Q8View& b, int metric, float* out, s
     if (q.n <= 16 && b.width() <= 4096) {                      // 64 KiB of LDS for the queries
         const uint32_t nb = b.blocks(), groups = (uint32_t)tiles_of(b.n, 16);
         const size_t lds = (size_t)nb * 2048 + (nb + 3) / 4 * 64;
-        // Few rows: a workgroup per 16 of them (kernel times: 10064 x 960 5.6 against 6.4 us, 2000 x 4096 8.5 against 15.5, but 100000 x 960
-        // 20.9 against 19.4).  The resident workgroups walk through the rest: 1M rows of 128 / 256 / 960 columns on 1024 workgroups 24.5 /
-        // 38.7 / 171 us, on 2048 23.1 / 41.0 / 187.
-        if (groups <= 2048 && nb >= 4) hipLaunchKernelGGL(stream_kernel<true>, dim3(groups), dim3(256), lds, s, q, b, metric, out, out_stride, groups);
-        else hipLaunchKernelGGL(stream_kernel<false>, dim3(std::min((groups + 3) / 4, nb == 1 ? 2048u : 1024u)), dim3(256), lds, s, q, b, metric, out, out_stride, groups);
+        // Few rows: a workgroup per 16 of them (10000 x 960 4.3 against 6.4 us, 2000 x 4096 7.3 against 15.5, but 50000 x 960 12.2 against 10.8).  The
+        // workgroups that walk through the rest, and the blocks that each wavefront has on its way or in work: 1M rows of 960 columns 162 us on
+        // 512 workgroups with 3, 176 on 1024, 174 on 768, 211 on 256 (fewer walks keep to fewer pages of memory; 2 blocks 167 / 178 / 170);
+        // 16 x 100000 x 4096 107 / 115 / 114; rows of one block 4 x 1M x 100 22 us on 1024 with 2, 27 on 512, 22 on 2048.
+        auto launch = [&](auto kind) {
+            constexpr int METRIC = decltype(kind)::value;
+            const uint32_t wanted = (groups + 3) / 4;
+            if (groups <= 2048 && nb >= 4) hipLaunchKernelGGL((stream_kernel<METRIC, true, 2>), dim3(groups), dim3(256), lds, s, q, b, out, out_stride, groups);
+            else if (nb == 1) hipLaunchKernelGGL((stream_kernel<METRIC, false, 2>), dim3(std::min(wanted, 1024u)), dim3(256), lds, s, q, b, out, out_stride, groups);
+            else hipLaunchKernelGGL((stream_kernel<METRIC, false, 3>), dim3(std::min(wanted, 512u)), dim3(256), lds, s, q, b, out, out_stride, groups);
+        };
+        if (metric == VDB_DOT) launch(std::integral_constant<int, VDB_DOT>{});
+        else if (metric == VDB_COSINE) launch(std::integral_constant<int, VDB_COSINE>{});
+        else launch(std::integral_constant<int, VDB_EUCLIDEAN>{});
         VDB_HIP(hipGetLastError());
         return;
     }
