@@ -613,7 +613,8 @@ gemm_kernel(Q8View q, Q8View b, int metric, float* __restrict__ out, size_t out_
 
 // Too few tiles for the kernel above: a workgroup scores 32 rows against 32 queries, its four wavefronts take a quarter of the columns
 // each, straight from memory to registers with the next block on its way, and add up in LDS, in one order.
-// It takes rows of any stride.
+// It takes rows of any stride.  Bound by what one compute unit can fetch (64 x 64 x 4096: 256 KB each on four of them in 12 us; 8 wavefronts
+// with an eighth of the columns 12.9, three blocks ahead 13.3, operands of 16 x 32 14.5).
 __global__ void __launch_bounds__(256) narrow_kernel(Q8View q, Q8View b, int metric, float* __restrict__ out, size_t out_stride, uint32_t row_tiles, uint64_t tiles) {
     __shared__ float part[4][16][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), r = lane & 31, g = lane >> 5;
@@ -625,16 +626,19 @@ __global__ void __launch_bounds__(256) narrow_kernel(Q8View q, Q8View b, int met
         const uint8_t* yc = q.codes + qu * q.cs; const uint8_t* ys = q.scales + qu * q.ss;
         floatx16 acc = {};
         struct Block { uint4 x[4], y[4]; uint32_t xs, ys; };
-        auto load = [&](Block& to, uint32_t k) {
+        auto load = [&](Block& to, uint32_t k) {               // on no condition: chunks behind a row's end repeat its last
             to.xs = xs[k]; to.ys = ys[k];
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
-                const uint32_t at = k * Q8_BLOCK + 32 * h + 16 * g;
-                to.x[h] = load16(xc, at, width); to.y[h] = load16(yc, at, width);
+                const uint32_t at = min(k * Q8_BLOCK + 32 * h + 16 * g, width - 16);
+                to.x[h] = *reinterpret_cast<const uint4*>(xc + at); to.y[h] = *reinterpret_cast<const uint4*>(yc + at);
             }
         };
-        auto multiply = [&](const Block& v) {
+        auto multiply = [&](Block& v, uint32_t k) {
             const float xf = scale_of(v.xs), yf = scale_of(v.ys);
+            if ((k + 1) * Q8_BLOCK > width)
+#pragma unroll
+                for (int h = 0; h < 4; ++h) if (k * Q8_BLOCK + 32 * h + 16 * g >= width) v.x[h] = v.y[h] = uint4{0, 0, 0, 0};
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
                 acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen(v.y[h].x, v.y[h].y, yf), widen(v.x[h].x, v.x[h].y, xf), acc, 0, 0, 0);
@@ -645,10 +649,10 @@ __global__ void __launch_bounds__(256) narrow_kernel(Q8View q, Q8View b, int met
         if (lo < hi) load(u, lo);
         for (uint32_t k = lo; k < hi; k += 2) {
             load(v, min(k + 1, hi - 1));
-            multiply(u);
+            multiply(u, k);
             if (k + 1 >= hi) break;
             load(u, min(k + 2, hi - 1));
-            multiply(v);
+            multiply(v, k + 1);
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) part[wave][e][lane] = acc[e];
