@@ -851,10 +851,13 @@ static void launch_gemm(const Q8View& q, const Q8View& b, int metric, float* out
         return std::max(cus * std::max(per_cu, 1), 8);
     }();
     const uint32_t grid = (uint32_t)std::min<uint64_t>(((uint64_t)rt * qt + 7) / 8, resident / 8) * 8;
-    // Scores that the last-level cache (256 MB) cannot keep leave with the streaming hint (1000 x 1M x 64: 784 against 853 us, 8000 x 125000 x 960
-    // 1837 against 2327, 64 x 1M x 64 54 against 71; but 3860 x 12928 x 84, 200 MB, 49 against 42), unless score rows begin inside a sector of
-    // 32 bytes, whose parts have to be joined (1000 x 1000002 x 64: 1358 against 1210, 128 x 200001 x 128 42 against 26).
-    const bool streaming = 4.0 * q.n * b.n > 235e6 && out_stride % 8 == 0 && (uintptr_t)out % 32 == 0;
+    // Scores that the last-level cache (256 MB) cannot keep leave with the streaming hint: they would drive the codes out of the L2 (1000 x 1M x
+    // 64: 784 against 853 us, 8000 x 125000 x 960 1837 against 2327, 64 x 1M x 64 54 against 71; but 3860 x 12928 x 84, 200 MB, 49 against 42).
+    // Score rows that share lines cost more that way, since their parts are not joined on the way, so there must be products enough to hide it
+    // and codes that are read again: 1024 x 154113 x 64 / 128 / 256 / 512 / 960 columns 270 / 264 / 252 / 246 / 390 us, without the hint 180 / 194 /
+    // 242 / 321 / 457; 678 x 729766 x 392 828 and 805, 64 x 1000003 x 960 332 and 309.
+    const bool lines = out_stride % 32 == 0 && (uintptr_t)out % 128 == 0;
+    const bool streaming = 4.0 * q.n * b.n > 235e6 && (lines || (b.width() >= 256 && q.n > 768));
     hipLaunchKernelGGL((gemm_kernel<BM, BN, WM, WN, S>), dim3(grid), dim3(THREADS), 0, s, q, b, metric, out, out_stride, TileOrder{rt, qt, std::min<uint32_t>(qt, 2048 / BN)},
                        streaming);
     VDB_HIP(hipGetLastError());

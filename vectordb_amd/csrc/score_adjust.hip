@@ -9,19 +9,18 @@ namespace {
 // A workgroup takes a span of columns of one query, four consecutive columns per thread and piece.  The scores are on their way while
 // the span's columns of the query's list are counted in LDS (integer atomics: the same counts in any order); then every score is
 // written once.  Bound by HBM: 8 bytes per column, 4 more for boosts.  Rows need no more than the alignment of a float.
-// Workgroups are dealt to the eight dies in turn: all queries of a span go to one die, one behind the other, so that a bitmap or a row
-// of boosts that they share is read once (16 x 1000003 with both: 22.4 us, query by query 28.3).
+// Workgroups are dealt to the eight dies in turn: each die takes an eighth of the spans of all queries, the queries of a span one behind
+// the other, so that a bitmap or a row of boosts that they share is read once (16 x 1000003 with both: 22.4 us, query by query 28.3).
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef floatx4 floatx4_u __attribute__((aligned(4)));
 
 template <int SPAN, int THREADS, bool SEEN>
-__global__ void __launch_bounds__(THREADS) adjust_kernel(AdjustArgs a, uint32_t spans, uint64_t tasks) {
+__global__ void __launch_bounds__(THREADS) adjust_kernel(AdjustArgs a, uint64_t tasks) {
     constexpr int PIECES = SPAN / (4 * THREADS);
     __shared__ uint4 count[SEEN ? SPAN / 4 : 1];
-    for (uint64_t t = blockIdx.x; t < tasks; t += gridDim.x) {
-        const uint64_t span = t / (8ull * a.nq) * 8 + t % 8;
-        if (span >= spans) continue;                           // of the whole workgroup
-        const uint32_t q = (uint32_t)(t / 8 % a.nq), lo = (uint32_t)span * SPAN, m = min((uint32_t)SPAN, a.n - lo);
+    const uint64_t per = (tasks + 7) / 8, end_task = min((blockIdx.x % 8 + 1) * per, tasks);
+    for (uint64_t t = blockIdx.x % 8 * per + blockIdx.x / 8; t < end_task; t += gridDim.x / 8) {
+        const uint32_t q = (uint32_t)(t % a.nq), lo = (uint32_t)(t / a.nq) * SPAN, m = min((uint32_t)SPAN, a.n - lo);
         const float* scores = a.scores + q * a.stride + lo;
         floatx4 g[PIECES];
 #pragma unroll
@@ -95,11 +94,10 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(AdjustArgs a, uint32_t 
 
 template <int SPAN, int THREADS>
 static void launch(const AdjustArgs& a, hipStream_t s) {
-    const uint32_t spans = (uint32_t)(((uint64_t)a.n + SPAN - 1) / SPAN);
-    const uint64_t tasks = ((uint64_t)spans + 7) / 8 * 8 * a.nq;
-    const dim3 grid((uint32_t)std::min<uint64_t>(tasks, 1u << 20));
-    if (a.how.seen) hipLaunchKernelGGL((adjust_kernel<SPAN, THREADS, true>), grid, dim3(THREADS), 0, s, a, spans, tasks);
-    else hipLaunchKernelGGL((adjust_kernel<SPAN, THREADS, false>), grid, dim3(THREADS), 0, s, a, spans, tasks);
+    const uint64_t tasks = ((uint64_t)a.n + SPAN - 1) / SPAN * a.nq;
+    const dim3 grid((uint32_t)std::min<uint64_t>((tasks + 7) / 8, 1u << 17) * 8);
+    if (a.how.seen) hipLaunchKernelGGL((adjust_kernel<SPAN, THREADS, true>), grid, dim3(THREADS), 0, s, a, tasks);
+    else hipLaunchKernelGGL((adjust_kernel<SPAN, THREADS, false>), grid, dim3(THREADS), 0, s, a, tasks);
     VDB_HIP(hipGetLastError());
 }
 
