@@ -214,7 +214,8 @@ SHAPES = [(1, 1, 1), (1, 15, 16), (2, 16, 17), (16, 17, 127), (17, 33, 128), (15
           (257, 1025, 768), (300, 77, 2000), (513, 600, 144), (1000, 130, 960), (7, 50, 9000), (5, 40, 4096), (16, 40000, 640), (3, 40, 4097), (2, 33, 4100), (70, 90, 4100), (130, 260, 4224), (1, 70000, 32), (500, 5000, 112),
           # each tile size of the tiled kernel, whole tiles and ragged ones
           (70, 20001, 300), (128, 12800, 64), (300, 60003, 70), (384, 51200, 128), (129, 50001, 200), (512, 25600, 192), (256, 65536, 16), (1000, 20003, 130),
-          (40, 150001, 70), (64, 153600, 48), (333, 2049, 200), (128, 8192, 128), (512, 131072, 16), (2000, 40001, 50), (128, 25600, 256)]
+          (40, 150001, 70), (64, 153600, 48), (333, 2049, 200), (128, 8192, 128), (512, 131072, 16), (2000, 40001, 50), (128, 25600, 256),
+          (33, 262145, 200), (64, 262144, 100), (128, 262144, 512), (90, 240001, 512)]
 
 
 @pytest.mark.parametrize("metric", list(M))
@@ -225,7 +226,7 @@ def test_scores_against_64_bits(vdb, metric, nq, n, dim):
 
 
 @pytest.mark.parametrize("metric", list(M))
-@pytest.mark.parametrize("nq,n", [(1, 333), (20, 333), (70, 333), (300, 333), (100, 20011), (129, 50001), (300, 60003), (600, 120000), (512, 131072), (200, 8001), (64, 150000)])
+@pytest.mark.parametrize("nq,n", [(1, 333), (20, 333), (70, 333), (300, 333), (100, 20011), (129, 50001), (300, 60003), (600, 120000), (512, 131072), (200, 8001), (64, 150000), (40, 262145)])
 def test_score_rows_lie_apart_and_what_is_between_stays(vdb, nq, n, metric):
     q, b = S.quantize_rows(gauss(nq, 200, 1).cuda()), S.quantize_rows(gauss(n, 200, 2).cuda())
     want = S.score_rows(q, b, metric)
@@ -273,7 +274,7 @@ def test_small_and_large_rows(vdb, nq, n, q_scale, b_scale):
         check_scores(S.score_rows(q, b, M.Euclidean), held(q), held(b), M.Euclidean, 200)
 
 
-@pytest.mark.parametrize("nq,n", [(2, 30), (40, 40), (300, 300), (100, 20000), (300, 60000), (200, 50000), (200, 8001), (64, 150000), (512, 131072)])
+@pytest.mark.parametrize("nq,n", [(2, 30), (40, 40), (300, 300), (100, 20000), (300, 60000), (200, 50000), (200, 8001), (64, 150000), (512, 131072), (33, 262145)])
 def test_nonfinite_rows_score_nan_and_no_others(vdb, nq, n):
     x, y = gauss(nq, 200, 1), gauss(n, 200, 2)
     x[1, 150] = float("inf"); y[3, 7] = float("nan"); y[n - 1, 199] = float("-inf")

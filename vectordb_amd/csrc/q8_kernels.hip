@@ -894,14 +894,15 @@ void launch_q8_score(const Q8View& q, const Q8View& b, int metric, float* out, s
         return;
     }
     // The larger the tile, the fewer conversions and LDS reads per product; the smaller, the more evenly tiles fall on the compute units
-    // and the sooner one is done.  With k tiles for the fullest of 256 compute units a size takes A + k w, in units of which a step of
-    // 64 columns scales both; A and w are fitted to 36 shapes and pick the fastest size or one at most 7 % behind it (16 % for 77 x 300007 x
-    // 100, whose last queries are half a tile).  In tiles of 256 x 256, 256 x 128, 128 x 128, 128 x 64 and 64 x 64, us:
+    // and the sooner one is done.  With k tiles for the fullest of 256 compute units and s steps of 64 columns a size takes about
+    // once + k (ends + s step) us; the figures are fitted to 126 shapes and pick a size that is 0.9 % behind the fastest on average and 13 % at
+    // most (1000 x 60000 x 100).  In tiles of 256 x 256, 256 x 128, 128 x 128, 128 x 64 and 64 x 64, us:
     //    678 x 729766 x  392   805   952  1088  1263  1423          64 x 1M     x 960   455  332  344  294  341
     //   1093 x 121956 x   77   145   137   167   178   204          20 x 100000 x 384    25   18   17   14   13
     //   1243 x   2485 x 3194    79    55    38    46    44         332 x 2060  x 1091    31   21   13   14   10
-    auto cost = [&](int bm, int bn, double once, double each) { return once + each * (double)((tiles_of(b.n, bm) * tiles_of(q.n, bn) + 255) / 256); };
-    const double costs[] = {cost(256, 256, 16, 42), cost(256, 128, 15, 21.5), cost(128, 128, 14, 11.2), cost(128, 64, 19, 8.4), cost(64, 64, 10.5, 5.5)};
+    const double steps = (b.width() + 63) / 64;
+    auto cost = [&](int bm, int bn, double once, double ends, double step) { return once + (double)((tiles_of(b.n, bm) * tiles_of(q.n, bn) + 255) / 256) * (ends + steps * step); };
+    const double costs[] = {cost(256, 256, 3.1, 4.9, 1.75), cost(256, 128, 2.8, 2.6, 1.04), cost(128, 128, 1.2, 1.35, 0.54), cost(128, 64, 4.4, 1.07, 0.32), cost(64, 64, 1.2, 0.66, 0.2)};
     switch (std::min_element(costs, costs + 5) - costs) {
         case 0: return launch_gemm<256, 256, 128, 64, 4>(q, b, metric, out, out_stride, s);
         case 1: return launch_gemm<256, 128, 64, 64, 4>(q, b, metric, out, out_stride, s);
