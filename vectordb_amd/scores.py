@@ -18,6 +18,7 @@ import torch
 from .capi import ArgumentError, DistanceMetric, Q8RowsC, ScoreAdjustC, VectorLengthMismatch
 
 BLOCK = 128                               # columns that share one scale
+_Tensor = torch.Tensor
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _METRICS = frozenset(int(m) for m in DistanceMetric)
 
@@ -43,28 +44,25 @@ def _refuse(why):
 
 def _check(t, what, dtype, ndim, device=None):
     """A tensor of one type and rank whose last axis is dense; -> elements from row to row."""
-    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.dim() != ndim:
+    if not isinstance(t, _Tensor) or t.dtype is not dtype or t.dim() != ndim:
         _refuse(f"{what}: expected a {ndim}-d {dtype} tensor")
     if device is not None and t.device != device:
         _refuse(f"{what} is on {t.device}, not on {device}")
-    shape, stride = t.shape, t.stride()
-    width = shape[-1]
-    if ndim == 2:
-        n = shape[0]
-        if n and width:
-            if width > 1 and stride[1] != 1:
-                _refuse(f"{what}: the last axis must be dense")
-            if n > 1:
-                if stride[0] < width:
-                    _refuse(f"{what}: rows overlap")
-                return stride[0]
-    elif width > 1 and stride[0] != 1:
+    width = t.shape[-1]
+    if t.is_contiguous():
+        return width
+    stride = t.stride()
+    if width > 1 and stride[-1] != 1:
         _refuse(f"{what}: the last axis must be dense")
+    if ndim == 2 and t.shape[0] > 1:
+        if stride[0] < width:
+            _refuse(f"{what}: rows overlap")
+        return stride[0]
     return width
 
 
 def _on_gpu(t, what):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    if not isinstance(t, _Tensor) or not t.is_cuda:
         _refuse(f"{what} must be a tensor on the GPU")
 
 
