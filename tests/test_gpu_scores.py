@@ -215,7 +215,9 @@ SHAPES = [(1, 1, 1), (1, 15, 16), (2, 16, 17), (16, 17, 127), (17, 33, 128), (15
           # each tile size of the tiled kernel, whole tiles and ragged ones
           (70, 20001, 300), (128, 12800, 64), (300, 60003, 70), (384, 51200, 128), (129, 50001, 200), (512, 25600, 192), (256, 65536, 16), (1000, 20003, 130),
           (40, 150001, 70), (64, 153600, 48), (333, 2049, 200), (128, 8192, 128), (512, 131072, 16), (2000, 40001, 50), (128, 25600, 256),
-          (33, 262145, 200), (64, 262144, 100), (128, 262144, 512), (90, 240001, 512)]
+          (33, 262145, 200), (64, 262144, 100), (128, 262144, 512), (90, 240001, 512),
+          # up to 32 queries
+          (17, 30000, 100), (32, 16000, 128), (31, 20001, 960), (17, 15000, 129), (32, 40000, 4096), (20, 33333, 300), (25, 14401, 4090)]
 
 
 @pytest.mark.parametrize("metric", list(M))
@@ -226,7 +228,7 @@ def test_scores_against_64_bits(vdb, metric, nq, n, dim):
 
 
 @pytest.mark.parametrize("metric", list(M))
-@pytest.mark.parametrize("nq,n", [(1, 333), (20, 333), (70, 333), (300, 333), (100, 20011), (129, 50001), (300, 60003), (600, 120000), (512, 131072), (200, 8001), (64, 150000), (40, 262145)])
+@pytest.mark.parametrize("nq,n", [(1, 333), (20, 333), (70, 333), (300, 333), (100, 20011), (129, 50001), (300, 60003), (600, 120000), (512, 131072), (200, 8001), (64, 150000), (40, 262145), (20, 20011), (32, 16000)])
 def test_score_rows_lie_apart_and_what_is_between_stays(vdb, nq, n, metric):
     q, b = S.quantize_rows(gauss(nq, 200, 1).cuda()), S.quantize_rows(gauss(n, 200, 2).cuda())
     want = S.score_rows(q, b, metric)
@@ -250,7 +252,7 @@ def test_rows_very_far_apart(vdb, nq, n):
     check_scores(S.score_rows(far, q, M.Euclidean), held(b), held(q), M.Euclidean, 300)
 
 
-@pytest.mark.parametrize("nq,n,dim", [(5, 40, 256), (40, 300, 256), (300, 300, 384), (100, 20000, 256), (300, 30000, 384), (200, 8001, 256), (64, 150000, 256), (500, 131072, 256)])
+@pytest.mark.parametrize("nq,n,dim", [(5, 40, 256), (40, 300, 256), (300, 300, 384), (100, 20000, 256), (300, 30000, 384), (200, 8001, 256), (64, 150000, 256), (500, 131072, 256), (20, 20000, 384), (32, 16000, 128)])
 def test_scales_far_apart(vdb, nq, n, dim):
     """Blocks from 2^-60 to 2^60 whose products meet in the middle."""
     g = torch.Generator().manual_seed(4)
@@ -274,7 +276,7 @@ def test_small_and_large_rows(vdb, nq, n, q_scale, b_scale):
         check_scores(S.score_rows(q, b, M.Euclidean), held(q), held(b), M.Euclidean, 200)
 
 
-@pytest.mark.parametrize("nq,n", [(2, 30), (40, 40), (300, 300), (100, 20000), (300, 60000), (200, 50000), (200, 8001), (64, 150000), (512, 131072), (33, 262145)])
+@pytest.mark.parametrize("nq,n", [(2, 30), (40, 40), (300, 300), (100, 20000), (300, 60000), (200, 50000), (200, 8001), (64, 150000), (512, 131072), (33, 262145), (20, 20000)])
 def test_nonfinite_rows_score_nan_and_no_others(vdb, nq, n):
     x, y = gauss(nq, 200, 1), gauss(n, 200, 2)
     x[1, 150] = float("inf"); y[3, 7] = float("nan"); y[n - 1, 199] = float("-inf")
@@ -286,7 +288,7 @@ def test_nonfinite_rows_score_nan_and_no_others(vdb, nq, n):
         assert torch.equal(torch.isnan(s), bad)
 
 
-@pytest.mark.parametrize("nq,n", [(1, 50), (9, 3000), (20, 70), (70, 20000), (300, 30000)])
+@pytest.mark.parametrize("nq,n", [(1, 50), (9, 3000), (20, 70), (70, 20000), (300, 30000), (20, 20000)])
 def test_bytes_behind_a_row_do_not_matter(vdb, nq, n):
     """NaN codes behind the row's 16-byte pieces, any scale behind its last block."""
     dim = 150

@@ -673,28 +673,30 @@ __global__ void __launch_bounds__(256) narrow_kernel(Q8View q, Q8View b, int met
     }
 }
 
-// Up to 16 queries: bound by the pass over the rows, which go from memory to registers.  The queries' codes lie in LDS, 16-byte chunk
+// Up to 16 or 32 queries (QT = 1, 2): bound by the pass over the rows, which go from memory to registers.  The queries' codes lie in LDS, 16-byte chunk
 // by chunk.  A wavefront takes 16 rows at a time, a block of 128 columns a step, and has DEPTH - 1 steps' codes on their way while it
 // multiplies one.  The queries are the left operand: a result register holds 16 rows of four queries.
 // Measured on 1 x 1M x 960: 162 us = 6.0 TB/s, 8 queries 195 (with rows staged through LDS, 4 wavefronts and 16 rows of 256 columns a step,
 // 160 and 188, but 45 instead of 23 on 1M x 128); 64 rows at a time 190 .. 212 us; with the streaming hint 190 us (the second half of a line
 // is fetched again).
 // SPLIT: the four wavefronts of a workgroup take a quarter of the columns each of the same rows and add up in LDS, in one order.
-template <int METRIC, bool SPLIT, int DEPTH>
-__global__ void __launch_bounds__(256) stream_kernel(Q8View q, Q8View b, float* __restrict__ out, size_t out_stride, uint32_t groups) {
-    extern __shared__ uint4 query[];                           // [8 chunks per block][16 queries], then the scales [4 blocks][16]
+template <int METRIC, bool SPLIT, int DEPTH, int QT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) stream_kernel(Q8View q, Q8View b, float* __restrict__ out, size_t out_stride, uint32_t groups) {
+    constexpr uint32_t NQ = 16 * QT, THREADS = 64 * WAVES;
+    static_assert(!SPLIT || QT == 1, "one part per wavefront");
+    extern __shared__ uint4 query[];                           // [8 chunks per block][NQ queries], then the scales [4 blocks][NQ]
     __shared__ floatx4 part[3][SPLIT ? 64 : 1];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), r = lane & 15, g = lane >> 4;
     const uint32_t nb = b.blocks(), width = b.width();
-    uint32_t* query_scale = reinterpret_cast<uint32_t*>(query + nb * 128);
-    for (uint32_t i = threadIdx.x; i < nb * 128; i += 256) query[i] = load16(q.codes + (size_t)min(i % 16, q.n - 1) * q.cs, i / 16 * 16, width);
-    for (uint32_t i = threadIdx.x; i < (nb + 3) / 4 * 16; i += 256) query_scale[i] = *reinterpret_cast<const uint32_t*>(q.scales + (size_t)min(i % 16, q.n - 1) * q.ss + i / 16 * 4);
+    uint32_t* query_scale = reinterpret_cast<uint32_t*>(query + nb * 8 * NQ);
+    for (uint32_t i = threadIdx.x; i < nb * 8 * NQ; i += THREADS) query[i] = load16(q.codes + (size_t)min(i % NQ, q.n - 1) * q.cs, i / NQ * 16, width);
+    for (uint32_t i = threadIdx.x; i < (nb + 3) / 4 * NQ; i += THREADS) query_scale[i] = *reinterpret_cast<const uint32_t*>(q.scales + (size_t)min(i % NQ, q.n - 1) * q.ss + i / NQ * 4);
     __syncthreads();
-    float nq[4];
+    float nq[4 * QT];                                          // register e of tile j: query 16 j + 4 g + e
 #pragma unroll
-    for (int e = 0; e < 4; ++e) nq[e] = norm_of(q.norms2, min(4 * g + e, q.n - 1), METRIC);
+    for (int e = 0; e < 4 * QT; ++e) nq[e] = norm_of(q.norms2, min(e / 4 * 16 + 4 * g + e % 4, q.n - 1), METRIC);
 
-    const uint32_t first_group = SPLIT ? blockIdx.x : blockIdx.x * 4 + wave, stride = SPLIT ? gridDim.x : gridDim.x * 4;
+    const uint32_t first_group = SPLIT ? blockIdx.x : blockIdx.x * WAVES + wave, stride = SPLIT ? gridDim.x : gridDim.x * WAVES;
     if (first_group >= groups) return;                         // SPLIT: of the whole workgroup
     // Loads are on no condition, or the compiler could not tell how many are on their way and would wait for all of them: rows behind the
     // last repeat it and are not stored, chunks behind a row's end repeat its last and meet zeros of the query.
@@ -711,22 +713,37 @@ __global__ void __launch_bounds__(256) stream_kernel(Q8View q, Q8View b, float* 
 #pragma unroll
         for (int h = 0; h < 2; ++h) to.v[h] = *reinterpret_cast<const uint4*>(row + min(k * Q8_BLOCK + 64 * h + 16 * g, width - 16));
     };
-    floatx4 acc{0.f, 0.f, 0.f, 0.f};
+    floatx4 acc[QT] = {};
     float norm;
     auto multiply = [&](const Step& x, uint32_t k) {
-        const float qs = scale_of(query_scale[k / 4 * 16 + r] >> (8 * (k & 3)) & 255u), rs = scale_of(x.scale);
+        float qs[QT];
+        const float rs = scale_of(x.scale);
+#pragma unroll
+        for (int j = 0; j < QT; ++j) qs[j] = scale_of(query_scale[k / 4 * NQ + 16 * j + r] >> (8 * (k & 3)) & 255u);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint4 v = query[(k * 8 + 4 * h + g) * 16 + r], w = x.v[h];
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(v.x, v.y, qs), widen(w.x, w.y, rs), acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(v.z, v.w, qs), widen(w.z, w.w, rs), acc, 0, 0, 0);
+            const uint4 w = x.v[h];
+            const bf16x8 lo = widen(w.x, w.y, rs), hi = widen(w.z, w.w, rs);
+#pragma unroll
+            for (int j = 0; j < QT; ++j) {
+                const uint4 v = query[(k * 8 + 4 * h + g) * NQ + 16 * j + r];
+                acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(v.x, v.y, qs[j]), lo, acc[j], 0, 0, 0);
+                acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(v.z, v.w, qs[j]), hi, acc[j], 0, 0, 0);
+            }
         }
+    };
+    auto clear = [&] {
+#pragma unroll
+        for (int j = 0; j < QT; ++j) acc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
     };
     auto store = [&](uint32_t group) {
         const uint64_t i = (uint64_t)group * 16 + r;
         if (i >= b.n) return;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) if (4 * g + e < q.n) out[(size_t)(4 * g + e) * out_stride + i] = finish(acc[e], nq[e], METRIC == VDB_COSINE ? root(norm) : norm, METRIC);
+        for (int e = 0; e < 4 * QT; ++e) {
+            const uint32_t at = e / 4 * 16 + 4 * g + e % 4;
+            if (at < q.n) out[(size_t)at * out_stride + i] = finish(acc[e / 4][e % 4], nq[e], METRIC == VDB_COSINE ? root(norm) : norm, METRIC);
+        }
     };
     auto load_norm = [&](uint32_t group) { norm = METRIC == VDB_DOT ? 0.f : b.norms2[row_at(group)]; };
     Step step[DEPTH];
@@ -736,7 +753,7 @@ __global__ void __launch_bounds__(256) stream_kernel(Q8View q, Q8View b, float* 
         for (uint32_t group = first_group; group < groups; group += stride) {
             go_to(group);
             load_norm(group);
-            acc = floatx4{0.f, 0.f, 0.f, 0.f};
+            clear();
             if (lo < hi) {
 #pragma unroll
                 for (int i = 0; i < DEPTH - 1; ++i) load(step[i], min(lo + i, hi - 1));
@@ -750,11 +767,11 @@ __global__ void __launch_bounds__(256) stream_kernel(Q8View q, Q8View b, float* 
                 }
             }
             __syncthreads();                                   // the parts of the last group are read
-            if (wave) part[wave - 1][lane] = acc;
+            if (wave) part[wave - 1][lane] = acc[0];
             __syncthreads();
             if (wave) continue;
 #pragma unroll
-            for (int w = 0; w < 3; ++w) acc += part[w][lane];
+            for (int w = 0; w < 3; ++w) acc[0] += part[w][lane];
             store(group);
         }
         return;
@@ -772,7 +789,7 @@ __global__ void __launch_bounds__(256) stream_kernel(Q8View q, Q8View b, float* 
         if (++k < nb) return false;
         k = 0;
         store(group);
-        acc = floatx4{0.f, 0.f, 0.f, 0.f};
+        clear();
         if (groups - group <= stride) return true;
         group += stride;
         load_norm(group);
@@ -863,32 +880,41 @@ static void launch_gemm(const Q8View& q, const Q8View& b, int metric, float* out
     VDB_HIP(hipGetLastError());
 }
 
+template <int METRIC>
+static void launch_stream(const Q8View& q, const Q8View& b, float* out, size_t out_stride, hipStream_t s) {
+    const uint32_t nb = b.blocks(), groups = (uint32_t)tiles_of(b.n, 16), sixteens = q.n > 16 ? 2 : 1;
+    const size_t lds = ((size_t)nb * 2048 + (nb + 3) / 4 * 64) * sixteens;
+    // Few rows: a workgroup per 16 of them (10000 x 960 4.3 against 6.4 us, 2000 x 4096 7.3 against 15.5, but 50000 x 960 12.2 against 10.8).  The
+    // workgroups that walk through the rest, and the blocks that each wavefront has on its way or in work: 1M rows of 960 columns 162 us on
+    // 512 workgroups with 3, 176 on 1024, 174 on 768, 211 on 256 (fewer walks keep to fewer pages of memory; 2 blocks 167 / 178 / 170);
+    // 16 x 100000 x 4096 107 / 115 / 114; rows of one block 4 x 1M x 100 22 us on 1024 with 2, 27 on 512, 22 on 2048.  32 queries of many
+    // columns leave room for one workgroup on a compute unit: 28 x 88422 x 3302 66 us on 256 of eight wavefronts, 86 on 512 of four.
+#define STREAM(SPLIT, DEPTH, QT, WAVES, MOST) \
+    hipLaunchKernelGGL((stream_kernel<METRIC, SPLIT, DEPTH, QT, WAVES>), dim3(std::min(SPLIT ? groups : (groups + WAVES - 1) / WAVES, MOST)), dim3(64 * WAVES), lds, s, q, b, out, out_stride, groups)
+    if (sixteens == 2) {
+        if (nb == 1) STREAM(false, 2, 2, 4, 1024u);
+        else STREAM(false, 2, 2, 8, 256u);
+    } else if (groups <= 2048 && nb >= 4) STREAM(true, 2, 1, 4, 2048u);
+    else if (nb == 1) STREAM(false, 2, 1, 4, 1024u);
+    else STREAM(false, 3, 1, 4, 512u);
+#undef STREAM
+    VDB_HIP(hipGetLastError());
+}
+
 void launch_q8_score(const Q8View& q, const Q8View& b, int metric, float* out, size_t out_stride, hipStream_t s) {
-    if (q.n <= 16 && b.width() <= 4096) {                      // 64 KiB of LDS for the queries
-        const uint32_t nb = b.blocks(), groups = (uint32_t)tiles_of(b.n, 16);
-        const size_t lds = (size_t)nb * 2048 + (nb + 3) / 4 * 64;
-        // Few rows: a workgroup per 16 of them (10000 x 960 4.3 against 6.4 us, 2000 x 4096 7.3 against 15.5, but 50000 x 960 12.2 against 10.8).  The
-        // workgroups that walk through the rest, and the blocks that each wavefront has on its way or in work: 1M rows of 960 columns 162 us on
-        // 512 workgroups with 3, 176 on 1024, 174 on 768, 211 on 256 (fewer walks keep to fewer pages of memory; 2 blocks 167 / 178 / 170);
-        // 16 x 100000 x 4096 107 / 115 / 114; rows of one block 4 x 1M x 100 22 us on 1024 with 2, 27 on 512, 22 on 2048.
-        auto launch = [&](auto kind) {
-            constexpr int METRIC = decltype(kind)::value;
-            const uint32_t wanted = (groups + 3) / 4;
-            if (groups <= 2048 && nb >= 4) hipLaunchKernelGGL((stream_kernel<METRIC, true, 2>), dim3(groups), dim3(256), lds, s, q, b, out, out_stride, groups);
-            else if (nb == 1) hipLaunchKernelGGL((stream_kernel<METRIC, false, 2>), dim3(std::min(wanted, 1024u)), dim3(256), lds, s, q, b, out, out_stride, groups);
-            else hipLaunchKernelGGL((stream_kernel<METRIC, false, 3>), dim3(std::min(wanted, 512u)), dim3(256), lds, s, q, b, out, out_stride, groups);
-        };
-        if (metric == VDB_DOT) launch(std::integral_constant<int, VDB_DOT>{});
-        else if (metric == VDB_COSINE) launch(std::integral_constant<int, VDB_COSINE>{});
-        else launch(std::integral_constant<int, VDB_EUCLIDEAN>{});
-        VDB_HIP(hipGetLastError());
-        return;
-    }
     const uint32_t rt = (uint32_t)tiles_of(b.n, 32);
     const uint64_t narrow = rt * tiles_of(q.n, 32);
+    // Queries for 64 (128) KiB of LDS.  17 to 32 of them against too few rows for all compute units are below (17 x 10000 x 960: 5.6 and 5.7 us, 32 x
+    // 5000 x 4096 13 and 27); against more 31 x 26096 x 3242 20 us instead of 37 in tiles, 20 x 20000 x 768 6.1 and 8.9, 32 x 1M x 960 229 and 258.
+    if (b.width() <= 4096 && (q.n <= 16 || (q.n <= 32 && narrow > 448))) {
+        if (metric == VDB_DOT) launch_stream<VDB_DOT>(q, b, out, out_stride, s);
+        else if (metric == VDB_COSINE) launch_stream<VDB_COSINE>(q, b, out, out_stride, s);
+        else launch_stream<VDB_EUCLIDEAN>(q, b, out, out_stride, s);
+        return;
+    }
     if (q.cs > MAX_STRIDE || b.cs > MAX_STRIDE || narrow <= 448) {
         // Times in tiles of 32 x 32 with split columns and of 64 x 64: 256 x 1000 x 4096 (256 of them) 13.1 and 26.0 us, 600 x 600 x 960 (361)
-        // 6.7 and 8.6, but 100 x 4000 x 2048 (500) 14.4 and 14.5, 20 x 20000 x 768 (625) 11.6 and 9.7.
+        // 6.7 and 8.6, but 100 x 4000 x 2048 (500) 14.4 and 14.5, 200 x 8000 x 768 (1750) 26 and 10.
         hipLaunchKernelGGL(narrow_kernel, dim3((uint32_t)std::min<uint64_t>(narrow, 1u << 20)), dim3(256), 0, s, q, b, metric, out, out_stride, rt, narrow);
         VDB_HIP(hipGetLastError());
         return;
