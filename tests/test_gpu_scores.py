@@ -217,7 +217,9 @@ SHAPES = [(1, 1, 1), (1, 15, 16), (2, 16, 17), (16, 17, 127), (17, 33, 128), (15
           (40, 150001, 70), (64, 153600, 48), (333, 2049, 200), (128, 8192, 128), (512, 131072, 16), (2000, 40001, 50), (128, 25600, 256),
           (33, 262145, 200), (64, 262144, 100), (128, 262144, 512), (90, 240001, 512),
           # up to 32 queries
-          (17, 30000, 100), (32, 16000, 128), (31, 20001, 960), (17, 15000, 129), (32, 40000, 4096), (20, 33333, 300), (25, 14401, 4090)]
+          (17, 30000, 100), (32, 16000, 128), (31, 20001, 960), (17, 15000, 129), (32, 40000, 4096), (20, 33333, 300), (25, 14401, 4090),
+          # few queries of many columns
+          (1, 300, 8192), (3, 33000, 8190), (16, 40001, 5000), (2, 70, 8193), (5, 33000, 9000)]
 
 
 @pytest.mark.parametrize("metric", list(M))

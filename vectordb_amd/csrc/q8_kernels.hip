@@ -682,16 +682,19 @@ __global__ void __launch_bounds__(256) narrow_kernel(Q8View q, Q8View b, int met
 // SPLIT: the four wavefronts of a workgroup take a quarter of the columns each of the same rows and add up in LDS, in one order.
 template <int METRIC, bool SPLIT, int DEPTH, int QT, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) stream_kernel(Q8View q, Q8View b, float* __restrict__ out, size_t out_stride, uint32_t groups) {
-    constexpr uint32_t NQ = 16 * QT, THREADS = 64 * WAVES;
+    constexpr uint32_t THREADS = 64 * WAVES;
     static_assert(!SPLIT || QT == 1, "one part per wavefront");
-    extern __shared__ uint4 query[];                           // [8 chunks per block][NQ queries], then the scales [4 blocks][NQ]
+    extern __shared__ uint4 query[];                           // [8 chunks per block][queries], then the scales [4 blocks][queries]
     __shared__ floatx4 part[3][SPLIT ? 64 : 1];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), r = lane & 15, g = lane >> 4;
     const uint32_t nb = b.blocks(), width = b.width();
-    uint32_t* query_scale = reinterpret_cast<uint32_t*>(query + nb * 8 * NQ);
-    for (uint32_t i = threadIdx.x; i < nb * 8 * NQ; i += THREADS) query[i] = load16(q.codes + (size_t)min(i % NQ, q.n - 1) * q.cs, i / NQ * 16, width);
-    for (uint32_t i = threadIdx.x; i < (nb + 3) / 4 * NQ; i += THREADS) query_scale[i] = *reinterpret_cast<const uint32_t*>(q.scales + (size_t)min(i % NQ, q.n - 1) * q.ss + i / NQ * 4);
+    uint32_t* query_scale = reinterpret_cast<uint32_t*>(query + nb * 8 * q.n);
+    for (uint32_t i = threadIdx.x; i < nb * 8 * q.n; i += THREADS) query[i] = load16(q.codes + (size_t)(i % q.n) * q.cs, i / q.n * 16, width);
+    for (uint32_t i = threadIdx.x; i < (nb + 3) / 4 * q.n; i += THREADS) query_scale[i] = *reinterpret_cast<const uint32_t*>(q.scales + (size_t)(i % q.n) * q.ss + i / q.n * 4);
     __syncthreads();
+    uint32_t mine[QT];                                         // this lane's query of each tile; those behind the last repeat it and are not stored
+#pragma unroll
+    for (int j = 0; j < QT; ++j) mine[j] = min(16 * j + r, q.n - 1);
     float nq[4 * QT];                                          // register e of tile j: query 16 j + 4 g + e
 #pragma unroll
     for (int e = 0; e < 4 * QT; ++e) nq[e] = norm_of(q.norms2, min(e / 4 * 16 + 4 * g + e % 4, q.n - 1), METRIC);
@@ -719,14 +722,14 @@ __global__ void __launch_bounds__(64 * WAVES) stream_kernel(Q8View q, Q8View b, 
         float qs[QT];
         const float rs = scale_of(x.scale);
 #pragma unroll
-        for (int j = 0; j < QT; ++j) qs[j] = scale_of(query_scale[k / 4 * NQ + 16 * j + r] >> (8 * (k & 3)) & 255u);
+        for (int j = 0; j < QT; ++j) qs[j] = scale_of(query_scale[k / 4 * q.n + mine[j]] >> (8 * (k & 3)) & 255u);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint4 w = x.v[h];
             const bf16x8 lo = widen(w.x, w.y, rs), hi = widen(w.z, w.w, rs);
 #pragma unroll
             for (int j = 0; j < QT; ++j) {
-                const uint4 v = query[(k * 8 + 4 * h + g) * NQ + 16 * j + r];
+                const uint4 v = query[(k * 8 + 4 * h + g) * q.n + mine[j]];
                 acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(v.x, v.y, qs[j]), lo, acc[j], 0, 0, 0);
                 acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(v.z, v.w, qs[j]), hi, acc[j], 0, 0, 0);
             }
@@ -882,20 +885,22 @@ static void launch_gemm(const Q8View& q, const Q8View& b, int metric, float* out
 
 template <int METRIC>
 static void launch_stream(const Q8View& q, const Q8View& b, float* out, size_t out_stride, hipStream_t s) {
-    const uint32_t nb = b.blocks(), groups = (uint32_t)tiles_of(b.n, 16), sixteens = q.n > 16 ? 2 : 1;
-    const size_t lds = ((size_t)nb * 2048 + (nb + 3) / 4 * 64) * sixteens;
-    // Few rows: a workgroup per 16 of them (10000 x 960 4.3 against 6.4 us, 2000 x 4096 7.3 against 15.5, but 50000 x 960 12.2 against 10.8).  The
-    // workgroups that walk through the rest, and the blocks that each wavefront has on its way or in work: 1M rows of 960 columns 162 us on
+    const uint32_t nb = b.blocks(), groups = (uint32_t)tiles_of(b.n, 16);
+    const size_t lds = ((size_t)nb * 128 + (nb + 3) / 4 * 4) * q.n;
+    // Few rows: a workgroup per 16 of them with split columns (16 x 2000 x 4096 8.8 us, 16 on 512 workgroups that walk on, 25 on 256; 1 x 5000 x 8192
+    // 14, 25 and 44; but 16 x 30000 x 2048 22.7, 15.6 and 13.7, 4 x 30000 x 960 7.4, 5.8 and 5.3).
+    // Workgroups that walk through the rows, and the blocks that each wavefront has on its way or in work: 1M rows of 960 columns 162 us on
     // 512 workgroups with 3, 176 on 1024, 174 on 768, 211 on 256 (fewer walks keep to fewer pages of memory; 2 blocks 167 / 178 / 170);
-    // 16 x 100000 x 4096 107 / 115 / 114; rows of one block 4 x 1M x 100 22 us on 1024 with 2, 27 on 512, 22 on 2048.  32 queries of many
-    // columns leave room for one workgroup on a compute unit: 28 x 88422 x 3302 66 us on 256 of eight wavefronts, 86 on 512 of four.
+    // 16 x 100000 x 4096 107 / 115 / 114; rows of one block 4 x 1M x 100 22 us on 1024 with 2, 27 on 512, 22 on 2048.  Many queries of
+    // many columns leave room for one workgroup on a compute unit: 28 x 88422 x 3302 66 us on 256 of eight wavefronts, 86 on 512 of four.
 #define STREAM(SPLIT, DEPTH, QT, WAVES, MOST) \
     hipLaunchKernelGGL((stream_kernel<METRIC, SPLIT, DEPTH, QT, WAVES>), dim3(std::min(SPLIT ? groups : (groups + WAVES - 1) / WAVES, MOST)), dim3(64 * WAVES), lds, s, q, b, out, out_stride, groups)
-    if (sixteens == 2) {
+    if (q.n > 16) {
         if (nb == 1) STREAM(false, 2, 2, 4, 1024u);
         else STREAM(false, 2, 2, 8, 256u);
-    } else if (groups <= 2048 && nb >= 4) STREAM(true, 2, 1, 4, 2048u);
+    } else if (groups <= 768 && nb >= 4) STREAM(true, 2, 1, 4, 768u);
     else if (nb == 1) STREAM(false, 2, 1, 4, 1024u);
+    else if (groups <= 4096 || lds > (80u << 10)) STREAM(false, 2, 1, 8, 256u);
     else STREAM(false, 3, 1, 4, 512u);
 #undef STREAM
     VDB_HIP(hipGetLastError());
@@ -904,9 +909,11 @@ static void launch_stream(const Q8View& q, const Q8View& b, float* out, size_t o
 void launch_q8_score(const Q8View& q, const Q8View& b, int metric, float* out, size_t out_stride, hipStream_t s) {
     const uint32_t rt = (uint32_t)tiles_of(b.n, 32);
     const uint64_t narrow = rt * tiles_of(q.n, 32);
-    // Queries for 64 (128) KiB of LDS.  17 to 32 of them against too few rows for all compute units are below (17 x 10000 x 960: 5.6 and 5.7 us, 32 x
-    // 5000 x 4096 13 and 27); against more 31 x 26096 x 3242 20 us instead of 37 in tiles, 20 x 20000 x 768 6.1 and 8.9, 32 x 1M x 960 229 and 258.
-    if (b.width() <= 4096 && (q.n <= 16 || (q.n <= 32 && narrow > 448))) {
+    // Queries for 128 KiB of LDS (1 x 100000 x 8192 188 us, in tiles of 64 x 64 259); where that is much for the few rows, and for 17 to 32 queries
+    // of few rows, the kernel below (16 x 10000 x 8192 56 against 34, 32 x 5000 x 4096 27 against 13, 17 x 10000 x 960 5.7 against 5.6; but 31 x 26096 x
+    // 3242 20 us and 37 in tiles, 20 x 20000 x 768 6.1 and 8.9, 32 x 1M x 960 229 and 258).
+    const uint64_t kib = (uint64_t)b.blocks() * q.n / 8;
+    if (kib <= 128 && q.n <= 32 && (narrow > 448 || (q.n <= 16 && kib <= 64))) {
         if (metric == VDB_DOT) launch_stream<VDB_DOT>(q, b, out, out_stride, s);
         else if (metric == VDB_COSINE) launch_stream<VDB_COSINE>(q, b, out, out_stride, s);
         else launch_stream<VDB_EUCLIDEAN>(q, b, out, out_stride, s);
