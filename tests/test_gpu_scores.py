@@ -219,7 +219,7 @@ SHAPES = [(1, 1, 1), (1, 15, 16), (2, 16, 17), (16, 17, 127), (17, 33, 128), (15
           # up to 32 queries
           (17, 30000, 100), (32, 16000, 128), (31, 20001, 960), (17, 15000, 129), (32, 40000, 4096), (20, 33333, 300), (25, 14401, 4090),
           # few queries of many columns
-          (1, 300, 8192), (3, 33000, 8190), (16, 40001, 5000), (2, 70, 8193), (5, 33000, 9000)]
+          (1, 300, 8192), (3, 33000, 8190), (16, 40001, 5000), (2, 70, 8193), (16, 14400, 8192), (1, 40, 131072), (1, 40, 131073)]
 
 
 @pytest.mark.parametrize("metric", list(M))

@@ -683,7 +683,7 @@ __global__ void __launch_bounds__(256) narrow_kernel(Q8View q, Q8View b, int met
 template <int METRIC, bool SPLIT, int DEPTH, int QT, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) stream_kernel(Q8View q, Q8View b, float* __restrict__ out, size_t out_stride, uint32_t groups) {
     constexpr uint32_t THREADS = 64 * WAVES;
-    static_assert(!SPLIT || QT == 1, "one part per wavefront");
+    static_assert(!SPLIT || (QT == 1 && WAVES == 4), "one part per wavefront");
     extern __shared__ uint4 query[];                           // [8 chunks per block][queries], then the scales [4 blocks][queries]
     __shared__ floatx4 part[3][SPLIT ? 64 : 1];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), r = lane & 15, g = lane >> 4;
