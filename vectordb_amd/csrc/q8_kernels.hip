@@ -813,10 +813,12 @@ __global__ void __launch_bounds__(64 * WAVES) stream_kernel(Q8View q, Q8View b, 
 }  // namespace
 
 template <class T, int LANES> static void launch_quantize_groups(const T* rows, size_t stride, const vdb_q8_rows& out, bool streaming, hipStream_t s) {
-    // A group per row while the grid allows, but rows of one block are over too soon for that (1M x 128: 142 against 130 us, 300007 x 100
-    // bf16: 31.5 against 29.1 on 8192 workgroups that walk on).
+    // A group per row while the grid allows, but rows of one or two blocks are over too soon for that.  In 2^16 / 2^17 / 2^18 / 2^21 groups that
+    // walk on: 1M x 128 124 / 120 / 115 / 126 us, 300007 x 100 bf16 19.4 / 19.2 / 20.1 / 20.8, 1M x 16 16.4 / 16.2 / 16.3 / 17.2; 771379 x 135 f32 128 / 127 /
+    // 128 / 139, 1M x 300 325 / 314 / 304 / 297.
     constexpr size_t per = 256 / LANES;
-    const uint32_t blocks = (uint32_t)std::min<size_t>((out.n + per - 1) / per, out.dim <= Q8_BLOCK ? 8192 : 1u << 18);
+    const size_t groups = out.dim <= Q8_BLOCK ? 1u << 17 : out.dim <= 2 * Q8_BLOCK ? 1u << 19 : 1u << 22;
+    const uint32_t blocks = (uint32_t)std::min((out.n + per - 1) / per, groups / per);
     if (streaming) hipLaunchKernelGGL((quantize_kernel<T, LANES, true>), dim3(blocks), dim3(256), 0, s, rows, stride, out);
     else hipLaunchKernelGGL((quantize_kernel<T, LANES, false>), dim3(blocks), dim3(256), 0, s, rows, stride, out);
     VDB_HIP(hipGetLastError());
