@@ -207,6 +207,41 @@ def test_more_rows_than_a_grid_holds(vdb):
     assert torch.equal(r.codes, want.codes[at]) and torch.equal(r.scales, want.scales[at]) and torch.equal(r.norms2, want.norms2[at])
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n,dim", [(19, 5), (19, 40), (19, 70), (2100, 150), (2100, 600), (2100, 520)])
+def test_any_alignment_and_a_larger_room_in_every_kernel(vdb, kind, n, dim):
+    """Rows at odd places of a wider table into rows of a wider room: the codes of dense rows, and nothing beside them."""
+    for at, pad in ((0, 0), (1, 2), (3, 8), (5, 0)):
+        wide = gauss(n, at + dim + pad, 5).to(TYPES[kind]).cuda()
+        wide[:, :at] = float("nan"); wide[:, at + dim:] = float("nan")
+        want = S.quantize_rows(wide[:, at:at + dim].clone())
+        w, sc = want.codes.shape[1], want.scales.shape[1]
+        room = S.Q8Rows(torch.full((n + 9, w + 16), 0xAB, dtype=torch.uint8, device="cuda"), torch.full((n + 9, sc + 4), 0xCD, dtype=torch.uint8, device="cuda"),
+                        torch.full((n + 9,), -1.0, device="cuda"), dim)
+        S.quantize_rows(wide[:, at:at + dim], out=room[4:4 + n])
+        assert torch.equal(room.codes[4:4 + n, :w], want.codes) and torch.equal(room.scales[4:4 + n, :sc], want.scales) and torch.equal(room.norms2[4:4 + n], want.norms2)
+        assert bool((room.codes[:4] == 0xAB).all()) and bool((room.codes[4 + n:] == 0xAB).all()) and bool((room.codes[:, w:] == 0xAB).all())
+        assert bool((room.scales[:4] == 0xCD).all()) and bool((room.scales[4 + n:] == 0xCD).all()) and bool((room.scales[:, sc:] == 0xCD).all())
+        assert bool((room.norms2[:4] == -1).all()) and bool((room.norms2[4 + n:] == -1).all())
+
+
+def test_more_long_rows_than_a_grid_holds(vdb):
+    """4.3 million rows of 520 bf16 values: more wavefronts than are launched, and bytes beyond 32 bits."""
+    n, dim, period = (4 << 20) + 99_991, 520, 1021
+    few = gauss(period, dim, 9).to(torch.bfloat16).cuda()
+    x = few[torch.arange(n, device="cuda") % period]
+    r, want = S.quantize_rows(x), S.quantize_rows(few.repeat(3, 1))                  # 3063 rows: the same kernel
+    del x
+    for lo in range(0, n, 1 << 20):
+        hi = min(n, lo + (1 << 20))
+        at = torch.arange(lo, hi, device="cuda") % period
+        assert torch.equal(r.codes[lo:hi], want.codes[at]) and torch.equal(r.scales[lo:hi], want.scales[at]) and torch.equal(r.norms2[lo:hi], want.norms2[at])
+    q = S.quantize_rows(gauss(40, dim, 4).cuda())                                    # tiles: the last rows against all of them
+    s = S.score_rows(q, r, M.Euclidean)
+    assert torch.equal(s[:, n - 3000:], S.score_rows(q, r, M.Euclidean)[:, n - 3000:])
+    check_scores(s[:, n - 200:], held(q), held(r[n - 200:]), M.Euclidean, dim)
+
+
 # ---------------------------------------------------------------- product
 
 SHAPES = [(1, 1, 1), (1, 15, 16), (2, 16, 17), (16, 17, 127), (17, 33, 128), (15, 64, 129), (3, 100, 100), (1, 1000, 960), (8, 1000, 960), (16, 999, 513),

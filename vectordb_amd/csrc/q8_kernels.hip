@@ -843,7 +843,7 @@ template <class T> static void launch_quantize(const T* rows, size_t stride, con
     // 271, but 1M x 384 384 and 326, f16 254 and 194 (a million wavefronts take 250 us to start; fewer that walk on are slower on long
     // rows: 65536 workgroups 860 us on 1M x 960, 2048 939).
     if (out.dim >= 512) {
-        const uint32_t blocks = (uint32_t)std::min<size_t>((out.n + 3) / 4, 1u << 22);
+        const uint32_t blocks = (uint32_t)std::min<size_t>((out.n + 3) / 4, 1u << 20);
         if (streaming) hipLaunchKernelGGL((quantize_wave_kernel<T, true>), dim3(blocks), dim3(256), 0, s, rows, stride, out);
         else hipLaunchKernelGGL((quantize_wave_kernel<T, false>), dim3(blocks), dim3(256), 0, s, rows, stride, out);
         VDB_HIP(hipGetLastError());
