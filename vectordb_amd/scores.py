@@ -83,14 +83,22 @@ def _out(out, nq, n, device):
 
 class Q8Rows:
     """Rows of `dim` columns as e4m3 codes (uint8 [n, >= dim, a multiple of 16]), one power-of-two scale per block of 128
-    columns (uint8 [n, >= blocks, a multiple of 4]: exponent + 127) and squared norms (f32 [n], or None: dot products only)."""
-    __slots__ = ("codes", "scales", "norms2", "dim", "_c")
+    columns (uint8 [n, >= blocks, a multiple of 4]: exponent + 127) and squared norms (f32 [n], or None: dot products only).
+    The attributes may be set anew: every call reads and checks the tensors that are there when it is made."""
+    __slots__ = ("codes", "scales", "norms2", "dim")
 
     def __init__(self, codes, scales, norms2, dim):
+        self.codes, self.scales, self.norms2, self.dim = codes, scales, norms2, int(dim)
+        self._c
+
+    @property
+    def _c(self):
+        """The tensors of this moment as the struct of the C ABI."""
+        codes, scales, norms2, dim = self.codes, self.scales, self.norms2, self.dim
         _on_gpu(codes, "codes")
         dev = codes.device
         cs, ss = _check(codes, "codes", torch.uint8, 2), _check(scales, "scales", torch.uint8, 2, dev)
-        (n, wide), (m, blocks), dim = codes.shape, scales.shape, int(dim)
+        (n, wide), (m, blocks) = codes.shape, scales.shape
         if dim < 1 or wide < -(-dim // 16) * 16 or blocks < -(-dim // (4 * BLOCK)) * 4:
             _refuse("codes or scales are narrower than a row")
         if m != n:
@@ -101,8 +109,7 @@ class Q8Rows:
             if norms2.shape[0] != n:
                 _refuse("codes and norms2 hold different numbers of rows")
             norms = norms2.data_ptr()
-        self.codes, self.scales, self.norms2, self.dim = codes, scales, norms2, dim
-        self._c = Q8RowsC(codes.data_ptr(), scales.data_ptr(), norms, n, dim, cs, ss)
+        return Q8RowsC(codes.data_ptr(), scales.data_ptr(), norms, n, dim, cs, ss)
 
     @classmethod
     def empty(cls, n, dim, device):
@@ -114,7 +121,6 @@ class Q8Rows:
         self.codes, self.scales = torch.empty((n, wide), dtype=torch.uint8, device=device), torch.empty((n, blocks), dtype=torch.uint8, device=device)
         self.norms2, self.dim = torch.empty(n, dtype=torch.float32, device=device), dim
         _on_gpu(self.codes, "a Q8Rows")
-        self._c = Q8RowsC(self.codes.data_ptr(), self.scales.data_ptr(), self.norms2.data_ptr(), n, dim, wide, blocks)
         return self
 
     def __len__(self):
@@ -137,10 +143,13 @@ def quantize_rows(rows, out=None):
     (n, dim), dev = rows.shape, rows.device
     if out is None:
         out = Q8Rows.empty(n, dim, dev)
-    elif len(out) != n or out.dim != dim or out.codes.device != dev:
+    elif not isinstance(out, Q8Rows):
+        _refuse("out is a Q8Rows")
+    to = out._c
+    if to.n != n or to.dim != dim or out.codes.device != dev:
         _refuse(f"out: expected {n} rows of {dim} columns on {dev}")
     api = _api()
-    api.check(api.fn.q8_quantize_dev(rows.data_ptr(), kind, stride, C.byref(out._c), _raw_stream(dev.index)))
+    api.check(api.fn.q8_quantize_dev(rows.data_ptr(), kind, stride, C.byref(to), _raw_stream(dev.index)))
     return out
 
 
@@ -148,14 +157,14 @@ def score_rows(queries, base, metric, out=None):
     """Scores [nq, n] of every query (Q8Rows) against every row (Q8Rows)."""
     if not isinstance(queries, Q8Rows) or not isinstance(base, Q8Rows):
         _refuse("queries and base are Q8Rows")
-    dev = base.codes.device
+    q, b, dev = queries._c, base._c, base.codes.device
     if queries.codes.device != dev:
         _refuse(f"queries are on {queries.codes.device}, not on {dev}")
-    if queries.dim != base.dim:
-        raise VectorLengthMismatch(f"Vector length mismatch: expected {base.dim}, got {queries.dim}")
-    out, stride = _out(out, queries._c.n, base._c.n, dev)
+    if q.dim != b.dim:
+        raise VectorLengthMismatch(f"Vector length mismatch: expected {b.dim}, got {q.dim}")
+    out, stride = _out(out, q.n, b.n, dev)
     api = _api()
-    api.check(api.fn.q8_score_dev(C.byref(queries._c), C.byref(base._c), _metric(metric), out.data_ptr(), stride, _raw_stream(dev.index)))
+    api.check(api.fn.q8_score_dev(C.byref(q), C.byref(b), _metric(metric), out.data_ptr(), stride, _raw_stream(dev.index)))
     return out
 
 
