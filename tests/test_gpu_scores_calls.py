@@ -68,3 +68,44 @@ def test_rows_that_no_longer_fit_are_refused(vdb, change):
     change(r)
     with pytest.raises(ArgumentError):
         S.score_rows(q, r, M.Dot)
+
+
+# ---------------------------------------------------------------- the call itself
+
+def test_a_small_adjustment_costs_about_one_torch_operation(vdb):
+    """Boosts on a thousand scores: a launch and little else, as the addition that it is.  The shortest of blocks taken in turn."""
+    import time
+    s, boost = torch.randn(1, 1000, device="cuda"), torch.randn(1000, device="cuda")
+    assert torch.equal(S.adjust_scores(s, M.Dot, boost=boost), s + boost)
+
+    def block(f, calls=300):
+        torch.cuda.synchronize()
+        t = time.perf_counter()
+        for _ in range(calls):
+            f()
+        torch.cuda.synchronize()
+        return time.perf_counter() - t
+    both = [(block(lambda: S.adjust_scores(s, M.Dot, boost=boost)), block(lambda: s + boost)) for _ in range(40)]
+    ours, torchs = min(a for a, _ in both), min(b for _, b in both)
+    assert ours <= 1.3 * torchs, (ours, torchs)
+
+
+def test_metrics_of_every_form(vdb):
+    import numpy as np
+    s = torch.randn(2, 40, device="cuda")
+    boost = torch.randn(40, device="cuda")
+    for m, want in ((0, s - boost), (1, s + boost), (2, s - boost)):
+        for form in (m, M(m), float(m), np.int64(m)):
+            assert torch.equal(S.adjust_scores(s, form, boost=boost), want)
+    for bad in (3, -1, 1 << 70, 0.5, None, "dot", [1], float("nan"), torch.tensor(1)):
+        with pytest.raises(ArgumentError):
+            S.adjust_scores(s, bad)
+
+
+def test_a_result_beyond_the_memory_is_torchs_own_error(vdb):
+    """Three terabytes of scores: refused by the allocator, and the next call works."""
+    q, b = S.Q8Rows.empty(200_000, 16, "cuda"), S.Q8Rows.empty(4_000_000, 16, "cuda")
+    with pytest.raises(torch.OutOfMemoryError):
+        S.score_rows(q, b, M.Dot)
+    x = gauss(3, 16, 1)
+    assert S.score_rows(S.quantize_rows(x), S.quantize_rows(x), M.Dot).shape == (3, 3)

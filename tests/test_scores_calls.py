@@ -20,3 +20,28 @@ def test_rows_keep_no_address(vdb):
     for call in (lambda: S.score_rows(r, r, 1), lambda: r._c):
         with pytest.raises(vdb.ArgumentError, match="codes"):                       # not an AttributeError: the tensors were looked at
             call()
+
+
+@pytest.mark.parametrize("call", [lambda: S.score_rows(1, 2), lambda: S.score_rows(1, 2, 3, 4, 5), lambda: S.score_rows(1, 2, 3, colour=4), lambda: S.score_rows(1, 2, 3, base=4),
+                                  lambda: S.quantize_rows(), lambda: S.quantize_rows(rows=1, rown=2), lambda: S.adjust_scores(1), lambda: S.adjust_scores(1, 2, 3), lambda: S.adjust_scores(1, 2, bost=3)])
+def test_calls_of_another_form_are_type_errors(call):
+    with pytest.raises(TypeError):
+        call()
+
+
+@pytest.mark.parametrize("call", [lambda r: S.quantize_rows(None), lambda r: S.quantize_rows(rows=torch.zeros(2, 4, device="meta")), lambda r: S.score_rows(r, 3, 1), lambda r: S.score_rows(base=r, queries=r, metric=1),
+                                  lambda r: S.adjust_scores([[1.0]], 1), lambda r: S.adjust_scores(metric=1, scores=torch.zeros(2, 2)), lambda r: S.Q8Rows.empty(3, 0, "cpu"), lambda r: S.Q8Rows.empty(-1, 8, "cpu"),
+                                  lambda r: S.Q8Rows.empty(3, 8, "cpu"), lambda r: S.Q8Rows(1, 2, 3, 4)])
+def test_what_is_no_tensor_on_the_gpu_is_refused(vdb, call):
+    with pytest.raises(vdb.ArgumentError):
+        call(host_rows(4))
+
+
+def test_the_calls_say_what_they_take():
+    import inspect
+    assert list(inspect.signature(S.quantize_rows).parameters) == ["rows", "out"]
+    assert list(inspect.signature(S.score_rows).parameters) == ["queries", "base", "metric", "out"]
+    p = inspect.signature(S.adjust_scores).parameters
+    assert list(p) == ["scores", "metric", "pass_bits", "boost", "seen", "seen_offsets", "repeat", "frequency", "presence", "out"]
+    assert all(p[k].kind is inspect.Parameter.KEYWORD_ONLY and p[k].default is None for k in list(p)[2:])
+    assert all(f.__doc__ for f in (S.quantize_rows, S.score_rows, S.adjust_scores))
