@@ -109,3 +109,94 @@ def test_a_result_beyond_the_memory_is_torchs_own_error(vdb):
         S.score_rows(q, b, M.Dot)
     x = gauss(3, 16, 1)
     assert S.score_rows(S.quantize_rows(x), S.quantize_rows(x), M.Dot).shape == (3, 3)
+
+
+# ---------------------------------------------------------------- gradients
+
+def test_what_requires_a_gradient_is_refused_while_gradients_are_recorded(vdb):
+    x = gauss(4, 32, 1).requires_grad_()
+    want = S.quantize_rows(x.detach())
+    with pytest.raises(ArgumentError, match="gradient"):
+        S.quantize_rows(x)
+    with pytest.raises(ArgumentError, match="gradient"):
+        S.quantize_rows(x * 2)
+    with torch.no_grad():
+        assert same(S.quantize_rows(x), want)
+    with torch.inference_mode():
+        assert same(S.quantize_rows(x), want)
+    # norms, scores and everything that is laid over them
+    r = S.Q8Rows(want.codes, want.scales, want.norms2, 32)
+    r.norms2 = want.norms2.clone().requires_grad_()
+    with pytest.raises(ArgumentError, match="gradient"):
+        S.score_rows(want, r, M.Cosine)
+    s, ones = torch.randn(4, 40, device="cuda"), torch.ones(4, device="cuda")
+    seen, off = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.arange(5, device="cuda")
+    lists = dict(seen=seen, seen_offsets=off)
+    kws = [dict(boost=torch.randn(40, device="cuda")), dict(repeat=ones, **lists), dict(frequency=ones, **lists), dict(presence=ones, **lists), dict(out=torch.empty_like(s))]
+    plain = [S.adjust_scores(s, M.Dot, **kw).clone() for kw in kws]
+    with pytest.raises(ArgumentError, match="gradient"):
+        S.adjust_scores(s.clone().requires_grad_(), M.Dot)
+    for kw, value in zip(kws, plain):
+        name = next(k for k in kw if k not in lists)
+        kw = {**kw, name: kw[name].clone().requires_grad_()}
+        with pytest.raises(ArgumentError, match="gradient"):
+            S.adjust_scores(s, M.Dot, **kw)
+        with torch.no_grad():
+            assert torch.equal(S.adjust_scores(s.clone().requires_grad_(), M.Dot, **kw), value)
+
+
+def test_an_output_that_a_backward_pass_saved_counts_as_changed(vdb):
+    a = torch.randn(3, 20, device="cuda", requires_grad=True)
+    s = a * 2
+    y = (s * s).sum()                                          # saves s
+    d = s.detach()
+    S.adjust_scores(d, M.Dot, boost=torch.ones(20, device="cuda"), out=d)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+
+
+def test_versions_of_outputs(vdb):
+    x = gauss(5, 40, 1)
+    r, s = S.quantize_rows(x), torch.empty(5, 5, device="cuda")
+    before = [t._version for t in (r.codes, r.scales, r.norms2, s, x)]
+    S.quantize_rows(x, out=r)
+    S.score_rows(r, r, M.Dot, out=s)
+    assert [t._version for t in (r.codes, r.scales, r.norms2, s, x)] == [v + 1 for v in before[:4]] + before[4:]
+    S.adjust_scores(s, M.Dot)
+    assert s._version == before[3] + 1
+    S.quantize_rows(x, out=S.Q8Rows(r.codes, r.scales, None, 40))
+    assert r.codes._version == before[0] + 2 and r.norms2._version == before[2] + 1
+    with torch.inference_mode():                               # such tensors have no versions
+        room, t = S.Q8Rows.empty(5, 40, "cuda"), torch.empty(5, 5, device="cuda")
+        S.quantize_rows(x, out=room)
+    S.score_rows(room, r, M.Dot, out=t)
+    assert same(room, S.quantize_rows(x)) and torch.equal(t, S.score_rows(r, r, M.Dot))
+
+
+def test_negated_views_and_tangents_are_refused(vdb):
+    import torch.autograd.forward_ad as fwad
+    x = gauss(4, 32, 1)
+    with pytest.raises(ArgumentError):
+        S.quantize_rows(torch._neg_view(x))
+    assert same(S.quantize_rows(torch._neg_view(x).resolve_neg()), S.quantize_rows(-x))
+    with pytest.raises(ArgumentError):
+        S.adjust_scores(x, M.Dot, out=torch._neg_view(x.clone()))
+    with fwad.dual_level():
+        with pytest.raises(ArgumentError):
+            S.adjust_scores(fwad.make_dual(x, torch.ones_like(x)), M.Dot)
+        with pytest.raises(ArgumentError):
+            S.adjust_scores(x, M.Dot, boost=fwad.make_dual(x[0], torch.ones_like(x[0])))
+
+
+def test_tensors_without_memory_are_refused(vdb):
+    x = gauss(4, 32, 1)
+    with pytest.raises(ArgumentError):
+        S.quantize_rows(torch.sparse_coo_tensor([[0], [1]], [1.0], (4, 32), device="cuda"))
+    with pytest.raises(ArgumentError):
+        torch.func.vmap(lambda t: S.adjust_scores(t, M.Dot))(torch.stack([x, x]))
+    with pytest.raises(ArgumentError):
+        torch.func.grad(lambda t: S.adjust_scores(t, M.Dot).sum())(x)
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        with pytest.raises(ArgumentError):
+            S.quantize_rows(torch.empty(4, 32, device="cuda"))

@@ -4,6 +4,7 @@
 // Nothing of a tensor is kept; the interpreter's lock is free while the entry point runs.
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
 
 #include <cstdint>
 #include <string>
@@ -122,6 +123,10 @@ Seen seen(const at::Tensor& t, const char* what, at::ScalarType type, int axes, 
     if (t.scalar_type() != type || t.dim() != axes || t.layout() != at::kStrided) refuse(w + ": expected a " + std::to_string(axes) + "-d " + text(type) + " tensor");
     if (device && t.device() != *device) refuse(w + " is on " + text(t.device()) + ", not on " + text(*device));
     if (!t.has_storage()) refuse(w + ": a tensor without memory");
+    if (t.is_neg()) refuse(w + ": the memory of a negated view holds other values; resolve_neg() gives its own");
+    // No gradient goes through these calls: a tensor that asks for one is not passed by without a word.
+    if (t.requires_grad() && c10::GradMode::is_enabled()) refuse(w + " requires a gradient, and the call has none: pass " + w + ".detach(), or call under torch.no_grad()");
+    if (t._fw_grad(0).defined()) refuse(w + " carries a tangent, and the call has none: pass its primal value");
     Seen s;
     s.width = t.size(axes - 1);
     s.rows = axes == 2 ? t.size(0) : 1;
@@ -194,6 +199,11 @@ Result result(PyObject* out, int64_t nq, int64_t n, const c10::Device& device) {
     r.o = Ref(out);
     return r;
 }
+// Written past autograd: a backward pass that saved the tensor has to learn of it.
+void written(PyObject* o) {
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 template <class F> void call(const c10::Device& device, F&& entry) {
     const Ref index(got(PyLong_FromLong(device.index())));
     const Ref stream(got(PyObject_CallOneArg(raw_stream, index.p)));
@@ -246,6 +256,8 @@ PyObject* quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args, PyO
                 refuse("out: expected " + std::to_string(x.rows) + " rows of " + std::to_string(x.width) + " columns on " + text(device));
         }
         call(device, [&](void* stream) { return quantize_dev(x.p, (vdb_dtype)kind, (size_t)x.stride, &r.c, stream); });
+        if (a.v[1] != Py_None)
+            for (PyObject* o : {r.codes.p, r.scales.p, r.norms2.p}) if (o != Py_None) written(o);
         return out.take();
     } catch (...) { return set_error(); }
 }
@@ -267,6 +279,7 @@ PyObject* score_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args, PyObje
         const int metric = metric_of(a.v[2]);
         Result out = result(a.v[3], (int64_t)q.c.n, (int64_t)b.c.n, b.device);
         call(b.device, [&](void* stream) { return score_dev(&q.c, &b.c, (vdb_metric)metric, (float*)out.s.p, (size_t)out.s.stride, stream); });
+        if (a.v[3] != Py_None) written(out.o.p);
         return out.o.take();
     } catch (...) { return set_error(); }
 }
@@ -314,6 +327,7 @@ PyObject* adjust_scores(PyObject*, PyObject* const* args, Py_ssize_t n_args, PyO
         how.presence = each(PRESENCE);
         Result out = result(a.v[OUT], nq, n, device);
         call(device, [&](void* stream) { return adjust_dev((const float*)s.p, (size_t)s.stride, (size_t)nq, (size_t)n, (vdb_metric)metric, &how, (float*)out.s.p, (size_t)out.s.stride, stream); });
+        if (a.v[OUT] != Py_None) written(out.o.p);
         return out.o.take();
     } catch (...) { return set_error(); }
 }
@@ -354,15 +368,17 @@ PyObject* bind(PyObject*, PyObject* args) {
 PyMethodDef methods[] = {
     {"quantize_rows", (PyCFunction)(void (*)(void))quantize_rows, METH_FASTCALL | METH_KEYWORDS,
      "quantize_rows($module, rows, out=None)\n--\n\n"
-     "f32 / f16 / bf16 rows [n, dim] -> Q8Rows (into `out` where given: appending is quantize_rows(new, out=room[n:n + k]))."},
+     "f32 / f16 / bf16 rows [n, dim] -> Q8Rows (into `out` where given: appending is quantize_rows(new, out=room[n:n + k])).\n"
+     "Not differentiable: rows that require a gradient are refused while gradients are recorded."},
     {"score_rows", (PyCFunction)(void (*)(void))score_rows, METH_FASTCALL | METH_KEYWORDS,
      "score_rows($module, queries, base, metric, out=None)\n--\n\n"
-     "Scores [nq, n] of every query (Q8Rows) against every row (Q8Rows)."},
+     "Scores [nq, n] of every query (Q8Rows) against every row (Q8Rows).  Not differentiable."},
     {"adjust_scores", (PyCFunction)(void (*)(void))adjust_scores, METH_FASTCALL | METH_KEYWORDS,
      "adjust_scores($module, scores, metric, *, pass_bits=None, boost=None, seen=None, seen_offsets=None, repeat=None, frequency=None, presence=None, out=None)\n--\n\n"
      "What vdb_score_adjust describes, over scores [nq, n] f32 (a tensor of its own, or `out`; out=scores works in place).\n\n"
      "pass_bits: int32 [words] or [1 or nq, words], words = ceil(n / 32); boost: f32 [n] or [1 or nq, n]; seen: int32 columns of all\n"
-     "queries behind each other (read as unsigned; those >= n are passed over), seen_offsets: int64 [nq + 1]; repeat / frequency / presence: f32 [nq]."},
+     "queries behind each other (read as unsigned; those >= n are passed over), seen_offsets: int64 [nq + 1]; repeat / frequency / presence: f32 [nq].\n"
+     "Not differentiable: tensors that require a gradient are refused while gradients are recorded."},
     {"rows_struct", (PyCFunction)(void (*)(void))rows_struct, METH_FASTCALL, "rows_struct($module, codes, scales, norms2, dim, /)\n--\n\nThe members of vdb_q8_rows for these tensors."},
     {"check_rows", (PyCFunction)(void (*)(void))check_rows, METH_FASTCALL, "check_rows($module, codes, scales, norms2, dim, /)\n--\n\nRefuses tensors that do not hold rows of `dim` columns."},
     {"bind", bind, METH_VARARGS, "bind($module, quantize, score, adjust, rows_class, check, refusal, length_mismatch, out_of_memory, raw_stream, metrics, /)\n--\n\nThe entry points' addresses and what belongs to them."},

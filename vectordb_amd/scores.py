@@ -8,6 +8,8 @@
 Each call is one entry point of the C ABI (vdb_q8_quantize_dev, vdb_q8_score_dev, vdb_score_adjust_dev: include/vdbmi.h has
 the formulas and the layout), enqueued on the current stream of the tensors' device; nothing waits.  Tensors must live on one
 GPU; what a call cannot take is refused with ArgumentError before anything is launched, or VectorLengthMismatch for rows of two lengths.
+The calls have no gradient: while gradients are recorded a tensor that requires one is refused, as are tensors with tangents and
+negated views; a tensor written through `out` counts as changed in place, so that a backward pass which saved it says so.
 The calls themselves are in the module _tensors (csrc/tensors.cpp): a small one is over in the time of a few Python statements.
 """
 from __future__ import annotations
