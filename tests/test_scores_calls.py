@@ -1,9 +1,12 @@
 """The tensor calls on 8-bit rows and score rows: what they read and refuse, on the host (CPU-safe)."""
+import ctypes as C
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
 from vectordb_amd import scores as S  # noqa: E402
+from vectordb_amd.capi import ScoreAdjustC  # noqa: E402
 
 
 def host_rows(n, dim=32):
@@ -45,3 +48,12 @@ def test_the_calls_say_what_they_take():
     assert list(p) == ["scores", "metric", "pass_bits", "boost", "seen", "seen_offsets", "repeat", "frequency", "presence", "out"]
     assert all(p[k].kind is inspect.Parameter.KEYWORD_ONLY and p[k].default is None for k in list(p)[2:])
     assert all(f.__doc__ for f in (S.quantize_rows, S.score_rows, S.adjust_scores))
+
+
+@pytest.mark.parametrize("n_seen", [1 << 60, 1 << 62, (1 << 62) + 1, (1 << 64) - 1])
+def test_a_list_beyond_the_address_space_is_refused(vdb, n_seen):
+    """4 n_seen bytes that wrap to a few must not pass for a short list."""
+    p = 1 << 20
+    how = ScoreAdjustC(n_seen=n_seen, seen=p + (1 << 31), seen_offsets=p + (1 << 32))
+    with pytest.raises(vdb.ArgumentError):
+        vdb.check(vdb.fn.score_adjust_dev(p, 100, 4, 100, 1, C.byref(how), p + (1 << 30), 100, None))

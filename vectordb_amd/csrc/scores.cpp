@@ -174,7 +174,7 @@ vdb_status vdb_score_adjust_dev(const float* d_scores, size_t stride, size_t nq,
         AdjustArgs a{d_scores, d_out, stride, out_stride, (uint32_t)nq, (uint32_t)n, metric != VDB_DOT, *how};
         if (!a.how.n_seen) a.how.seen = nullptr;
         if (!a.how.seen) { a.how.seen_offsets = nullptr; a.how.repeat = a.how.frequency = a.how.presence = nullptr; }
-        for (size_t v : {stride, out_stride, how->pass_stride, how->boost_stride}) if (v >> 60) throw Failure(err_arg("a stride does not fit the address space"));
+        for (size_t v : {stride, out_stride, how->pass_stride, how->boost_stride, how->n_seen}) if (v >> 60) throw Failure(err_arg("a stride or n_seen does not fit the address space"));
         const Range o = range_of(d_out, nq, n * 4, out_stride * 4, "d_out"), in = range_of(d_scores, nq, n * 4, stride * 4, "d_scores");
         if (meet(o, in) && !(d_out == d_scores && out_stride == stride)) throw Failure(err_arg("d_out overlaps d_scores"));
         const size_t each = nq, one = 1;
