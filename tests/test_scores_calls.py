@@ -57,3 +57,15 @@ def test_a_list_beyond_the_address_space_is_refused(vdb, n_seen):
     how = ScoreAdjustC(n_seen=n_seen, seen=p + (1 << 31), seen_offsets=p + (1 << 32))
     with pytest.raises(vdb.ArgumentError):
         vdb.check(vdb.fn.score_adjust_dev(p, 100, 4, 100, 1, C.byref(how), p + (1 << 30), 100, None))
+
+
+def test_the_module_alone_raises_and_does_not_crash():
+    """Its functions before vectordb_amd.scores has given it the entry points."""
+    import os
+    import subprocess
+    import sys
+    calls = ["quantize_rows(1)", "score_rows(1, 2, 3)", "adjust_scores(1, 2)", "check_rows(1, 2, 3, 4)", "rows_struct(1, 2, 3, 4)", "check_rows(1)", "bind()"]
+    code = "import torch\nfrom vectordb_amd import _tensors as t\n" + "".join("try:\n    t.%s\nexcept (RuntimeError, TypeError):\n    print('raised', flush=True)\n" % c for c in calls)
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.split() == ["raised"] * len(calls), (r.returncode, r.stdout, r.stderr[-500:])

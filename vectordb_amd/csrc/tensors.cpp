@@ -55,6 +55,7 @@ PyObject* set_error() {                                        // the exception 
 template <int N> struct Arguments {
     PyObject* v[N];
     Arguments(const char* call, const char* const (&names)[N], PyObject* (&interned)[N], int needed, int by_place, PyObject* const* args, Py_ssize_t n, PyObject* kwnames) {
+        if (!rows_class) { PyErr_SetString(PyExc_RuntimeError, "vectordb_amd.scores has to be imported first"); throw Raised{}; }
         if (n > by_place) { PyErr_Format(PyExc_TypeError, "%s() takes at most %d positional arguments (%zd given)", call, by_place, n); throw Raised{}; }
         for (int i = 0; i < N; ++i) v[i] = i < n ? args[i] : nullptr;
         const Py_ssize_t named = kwnames ? PyTuple_GET_SIZE(kwnames) : 0;
