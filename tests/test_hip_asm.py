@@ -25,11 +25,9 @@ def statements():
             yield os.path.basename(path), text[m.end():i - 1]
 
 
-def parts(statement):
-    """-> instructions, the list of what is overwritten."""
+def instructions(statement):
     code = " ".join(re.findall(r'"((?:[^"\\]|\\.)*)"', statement.split(":")[0])).replace("\\n", "\n").replace("\\t", " ")
-    sections = re.split(r":(?![^()]*\))", statement)
-    return [x.strip() for x in code.split("\n") if x.strip()], sections[3] if len(sections) > 3 else ""
+    return [x.strip() for x in code.split("\n") if x.strip()]
 
 
 def test_there_are_statements_to_look_at():
@@ -37,10 +35,12 @@ def test_there_are_statements_to_look_at():
 
 
 @pytest.mark.parametrize("name,statement", list(statements()))
-def test_what_is_written_is_named_and_waits_are_long_enough(name, statement):
-    code, overwritten = parts(statement)
-    if any(re.match(r"s_mov_b32 m0\b", x) for x in code):
-        assert '"m0"' in overwritten, (name, statement)
+def test_m0_is_put_back_and_waits_are_long_enough(name, statement):
+    code = instructions(statement)
+    if any(re.match(r"s_mov_b32 m0\b", x) for x in code):     # the compiler reserves m0 and takes no note of it in a list of overwritten registers
+        kept = re.match(r"s_mov_b32 (%\d+), m0$", code[0])
+        assert kept and code[-1] == "s_mov_b32 m0, " + kept[1], (name, statement)
+        assert not any(kept[1] in re.findall(r"%\d+", x) for x in code[1:-1]), (name, statement)
     for i, x in enumerate(code):
         if not x.startswith("global_load_lds"):
             continue
