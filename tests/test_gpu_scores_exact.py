@@ -115,6 +115,25 @@ def test_long_sums_of_positive_products(vdb, nq, n, dim):
     assert torch.equal(S.score_rows(rows_of(q), rows_of(b), M.Dot).double(), products(q, b))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("metric", list(M))
+@pytest.mark.parametrize("nq,n,dim", [(600, 100003, 300), (300, 200001, 960), (1000, 60001, 272), (640, 100000, 256)])
+def test_large_score_matrices_whose_rows_share_lines(vdb, nq, n, dim, metric):
+    """Scores beyond the last-level cache, in rows that begin anywhere in a line: those of dense aligned rows, and nothing between them."""
+    g = generator(7)
+    q, b = (S.quantize_rows(torch.randn(k, dim, generator=g, device="cuda")) for k in (nq, n))
+    wide = -(-n // 32) * 32 + 64
+    aligned = torch.full((nq, wide), -5.0, device="cuda")
+    S.score_rows(q, b, metric, out=aligned[:, :n])
+    assert torch.equal(S.score_rows(q, b, metric), aligned[:, :n])
+    for at, apart in ((1, n + 3), (7, n + 8 + -n % 8)):
+        room = torch.full((nq, apart + 8), -5.0, device="cuda")
+        S.score_rows(q, b, metric, out=room[:, at:at + n])
+        assert torch.equal(room[:, at:at + n], aligned[:, :n])
+        assert bool((room[:, :at] == -5).all()) and bool((room[:, at + n:] == -5).all())
+    assert bool((aligned[:, n:] == -5).all())
+
+
 def test_a_window_of_13_bits_would_show():
     """The inputs above against a sum that keeps, of each eight products, 13 bits below the largest: nearly every score is another."""
     g = torch.Generator().manual_seed(1)

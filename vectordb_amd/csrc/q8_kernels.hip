@@ -885,10 +885,19 @@ static void launch_gemm(const Q8View& q, const Q8View& b, int metric, float* out
     // Scores that the last-level cache (256 MB) cannot keep leave with the streaming hint: they would drive the codes out of the L2 (1000 x 1M x
     // 64: 784 against 853 us, 8000 x 125000 x 960 1837 against 2327, 64 x 1M x 64 54 against 71; but 3860 x 12928 x 84, 200 MB, 49 against 42).
     // Score rows that share lines cost more that way, since their parts are not joined on the way, so there must be products enough to hide it
-    // and codes that are read again: 1024 x 154113 x 64 / 128 / 256 / 512 / 960 columns 270 / 264 / 252 / 246 / 390 us, without the hint 180 / 194 /
-    // 242 / 321 / 457; 678 x 729766 x 392 828 and 805, 64 x 1000003 x 960 332 and 309.
+    // (more than four steps of columns) and codes that are read again: by the next queries' tiles, or from the cache if they fit there.
+    // us without and with the hint, rows of 154113, 300007 and 729766 scores:
+    //    154113 columns  100        256        320        960    |  729766 columns  100        256        320        512        960
+    //      500      88   105   102   109   117   113   191   175 |    300       226   309   314   306   401   392   449   446   723   734
+    //      768     136   168   145   172   166   175   280   261 |    512                                531   507   578   575   876   897
+    //     1024     196   224   212   229   242   233   385   332 |    678       538   642   547   660   700   669   768   762  1223  1197
+    //     4000     745   845   819   848   945   855  1516  1212 |   2000      1781  1950  1930  1947  2279  1972
+    //    300007 columns  320        512        960       2000
+    //      200     100    92   115   108   175   190   337   338
+    //      384     196   187   206   180   328   349   608   630
+    //      512     227   224   250   240   374   386   658   667
     const bool lines = out_stride % 32 == 0 && (uintptr_t)out % 128 == 0;
-    const bool streaming = 4.0 * q.n * b.n > 235e6 && (lines || (b.width() >= 256 && q.n > 768));
+    const bool streaming = 4.0 * q.n * b.n > 235e6 && (lines || (b.width() > 256 && (q.n > 512 || (double)b.width() * b.n < 235e6)));
     hipLaunchKernelGGL((gemm_kernel<BM, BN, WM, WN, S>), dim3(grid), dim3(THREADS), 0, s, q, b, metric, out, out_stride, TileOrder{rt, qt, std::min<uint32_t>(qt, 2048 / BN)},
                        streaming);
     VDB_HIP(hipGetLastError());
