@@ -353,20 +353,17 @@ __device__ const uint4 zero16[1] = {};
 
 // A wavefront's load straight to LDS: lane i's BYTES bytes at base + off (p) go to dst + i * BYTES.  Written as assembly because the
 // compiler makes every LDS read behind such a load wait for it, whatever buffer it goes to; step_barrier() waits for the right ones.
-// m0 holds the LDS address; the compiler reserves it and takes no note of it as overwritten, so it is put back (the load has read it when it
-// is issued).  The compiler sees no instruction in here, so the waits are written out: one state between m0 and the load, and five before a
-// load that takes its base from scalar registers, which a vector instruction (v_readfirstlane) may have written last.
+// m0 holds the LDS address: an operand, so the compiler puts it there and knows that it did.  It sees no instruction in here, so the waits are
+// written out: one state between m0 and the load, and five before a load that takes its base from scalar registers, which a vector
+// instruction (v_readfirstlane) may have written last.
 __device__ inline void load16_to_lds(const uint8_t* base, uint32_t off, uint32_t dst) {
-    uint32_t m0;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 2\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0" : "=&s"(m0) : "v"(off), "s"(base), "s"(dst) : "memory");
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "{m0}"(dst) : "memory");
 }
 __device__ inline void load16_to_lds(const void* p, uint32_t dst) {
-    uint32_t m0;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0" : "=&s"(m0) : "v"(p), "s"(dst) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(p), "{m0}"(dst) : "memory");
 }
 __device__ inline void load4_to_lds(const void* p, uint32_t dst) {
-    uint32_t m0;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0" : "=&s"(m0) : "v"(p), "s"(dst) : "memory");
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(p), "{m0}"(dst) : "memory");
 }
 __device__ inline uint32_t lds_address(const void* p) {        // the same for the whole wavefront
     return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p);
