@@ -174,7 +174,8 @@ vdb_status vdb_q8_quantize_dev(const void* d_rows, vdb_dtype dtype, size_t strid
  * 1 - dot / (|q||i| + 1e-10); sqrt(max(0, |q|^2 + |i|^2 - 2 dot)) - the last one loses the digits that |q|^2 + |i|^2 and
  * 2 dot share.  Products are exact, sums are held in 32 bits; sums below 2^-126 may count as zero.  out_stride >= base->n; d_out must not overlap the rows. */
 vdb_status vdb_q8_score_dev(const vdb_q8_rows* queries, const vdb_q8_rows* base, vdb_metric metric, float* d_out, size_t out_stride, void* stream);
-/* vdb_score_scan over 8-bit rows: host buffers in f32, quantised and scored on `device`, out[q * n + i]. */
+/* vdb_score_scan over 8-bit rows: host buffers in f32, quantised and scored on `device`, out[q * n + i].  The f32 rows of the longer side, the
+ * codes of both and all nq * n scores are on the device at once; what does not fit is VDB_ERR_DEVICE. */
 vdb_status vdb_q8_score_scan(const float* queries, size_t nq, const float* base, size_t n, size_t dim, vdb_metric metric, int device, float* out);
 
 /* ---------------------------------------------------------------- score rows ---------------

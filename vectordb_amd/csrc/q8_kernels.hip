@@ -22,7 +22,7 @@ typedef short s16x2 __attribute__((ext_vector_type(2)));
 // every value held is an ordinary bf16 and f32 number; at e = 120 codes end at 240, so that no value rounds up to 2^128.
 // A lane reads 16 bytes, so 32 (16) lanes hold a block.  A row belongs to a group of that many lanes or fewer, to a wavefront or to a
 // workgroup, by its length and the number of rows; the next 16 bytes are on their way while some are converted.
-// Bound by HBM: 4 (2) bytes read, 1 + 1/128 written per column.  1M x 960 f32 837 us = 5.75 TB/s, 300007 x 100 bf16 20 us = 4.8 TB/s (rows
+// Bound by HBM: 4 (2) bytes read, 1 + 1/128 written per column.  1M x 960 f32 841 us = 5.7 TB/s, 300007 x 100 bf16 18 us = 5.1 TB/s (rows
 // of 100 columns leave lanes without work and lines in parts).  Few instructions count for short rows: with every value tested for
 // being finite and scaled by a multiplication of its own, 300007 x 128 bf16 took 27 us, 1M x 128 f16 75 instead of 64.
 
@@ -345,8 +345,8 @@ __device__ inline float finish(float dot, float nq, float nb, int metric) {
 // holds 32 rows of two queries.  Slot 32 i + r of WM holds row MT r + i (MT = WM / 32), so that MT registers of a lane are consecutive
 // rows: a store writes 128 MT bytes in a row for each of two queries.
 // The scales of four blocks are one word per row, which comes with every step.
-// Bound by power where products prevail (4096 x 32000 x 4096: 880 .. 920 us = 1.2 PFLOP/s, the matrix pipes busy 63 % of the time at 1.9 GHz; 766 us with
-// codes that are all equal), by the scores that leave where rows are short (1000 x 1M x 960: 2.06 ms, 4 GB of them).  On the first of these 16 x 16
+// Bound by power where products prevail (4096 x 32000 x 4096: 875 .. 940 us by card and warmth = 1.14 .. 1.23 PFLOP/s, the matrix pipes busy 63 % of the time at 1.9 GHz; 766 us with
+// codes that are all equal), by the scores that leave where rows are short (1000 x 1M x 960: 2.07 .. 2.2 ms, 4 GB of them).  On the first of these 16 x 16
 // instructions spill, and two workgroups of 256 x 128 per compute unit are slower; rings of 6, 9 and 12 buffers gain nothing on smaller tiles,
 // nor does letting a tile's stores go on through the next tile's first two steps.
 __device__ const uint4 zero16[1] = {};
