@@ -200,3 +200,17 @@ def test_tensors_without_memory_are_refused(vdb):
     with FakeTensorMode(allow_non_fake_inputs=True) as mode:
         with pytest.raises(ArgumentError):
             S.quantize_rows(torch.empty(4, 32, device="cuda"))
+
+
+def test_a_scan_beyond_the_memory_leaves_nothing_behind(vdb):
+    """A terabyte of rows is refused by the allocator before anything is read, and the next calls know nothing of it."""
+    import numpy as np
+    x = gauss(3, 64, 1)
+    want = S.score_rows(S.quantize_rows(x), S.quantize_rows(x), M.Dot)
+    room = np.zeros((4, 64), np.float32)
+    for _ in range(2):
+        with pytest.raises(vdb.DeviceError):
+            vdb.check(vdb.fn.q8_score_scan(room.ctypes.data, 1, room.ctypes.data, 4_000_000_000, 64, 1, 0, room.ctypes.data))
+        assert torch.equal(S.score_rows(S.quantize_rows(x), S.quantize_rows(x), M.Dot), want)
+        h = x.cpu().numpy()
+        assert np.array_equal(vdb.q8_score_scan(h, h, 1), want.cpu().numpy())

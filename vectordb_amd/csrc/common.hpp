@@ -35,11 +35,14 @@ struct Failure : std::exception {
     const char* what() const noexcept override { return e.msg.c_str(); }
 };
 
+// The error that is reported is taken off the thread, or the check behind the next launch would report it again.
 #define VDB_HIP(expr)                                                                                   \
     do {                                                                                                \
         hipError_t _e = (expr);                                                                         \
-        if (_e != hipSuccess)                                                                           \
+        if (_e != hipSuccess) {                                                                         \
+            (void)hipGetLastError();                                                                    \
             throw ::vdb::Failure(::vdb::err_device(std::string(#expr) + ": " + hipGetErrorString(_e))); \
+        }                                                                                               \
     } while (0)
 
 void set_last_error(const std::string& s);
