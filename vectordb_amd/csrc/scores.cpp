@@ -4,6 +4,7 @@
 #include "guard.hpp"
 #include "index.hpp"
 #include "q8.hpp"
+#include "scores_on.hpp"
 
 using namespace vdb;
 
@@ -21,18 +22,20 @@ Range range_of(const void* p, size_t n, size_t row, size_t stride, const char* w
 }
 bool meet(const Range& a, const Range& b) { return a.first < b.last && b.first < a.last; }
 
-// The device that owns every buffer of a call; the thread's current device is put back at the end.
+// The device that owns every buffer of a call; the thread's current device is put back at the end.  A caller that knows the device names
+// it, and the runtime is not asked about each buffer (60 ns each).
 class OnDevice {
 public:
-    OnDevice() {
+    explicit OnDevice(int known) : dev(known), ask(known < 0) {
         int n = 0;
-        if (hipGetDeviceCount(&n) != hipSuccess || n <= 0) { (void)hipGetLastError(); throw Failure(err_device("no HIP device available; libvdbmi has no CPU path")); }
+        if (ask && (hipGetDeviceCount(&n) != hipSuccess || n <= 0)) { (void)hipGetLastError(); throw Failure(err_device("no HIP device available; libvdbmi has no CPU path")); }
         VDB_HIP(hipGetDevice(&before));
     }
     ~OnDevice() { if (at >= 0 && at != before) (void)hipSetDevice(before); }
     OnDevice(const OnDevice&) = delete;
     OnDevice& operator=(const OnDevice&) = delete;
     void add(const void* p, const char* what) {
+        if (!ask) return;
         hipPointerAttribute_t a{};
         if (hipPointerGetAttributes(&a, p) != hipSuccess) { (void)hipGetLastError(); throw Failure(err_arg(std::string(what) + " is not device memory")); }
         if (a.type == hipMemoryTypeUnregistered) throw Failure(err_arg(std::string(what) + " is not device memory"));
@@ -42,7 +45,8 @@ public:
     }
     void enter() { if (dev >= 0 && dev != before) { VDB_HIP(hipSetDevice(dev)); at = dev; } }
 private:
-    int before = 0, dev = -1, at = -1;
+    int before = 0, dev, at = -1;
+    bool ask;
 };
 
 void check_rows(const vdb_q8_rows* r, const char* who) {
@@ -80,7 +84,7 @@ vdb_status vdb_q8_strides(size_t dim, size_t* code_stride, size_t* scale_stride)
     });
 }
 
-vdb_status vdb_q8_quantize_dev(const void* d_rows, vdb_dtype dtype, size_t stride, const vdb_q8_rows* out, void* stream) {
+vdb_status vdb_q8_quantize_on(int device, const void* d_rows, vdb_dtype dtype, size_t stride, const vdb_q8_rows* out, void* stream) {
     return guard([&] {
         check_rows(out, "out");
         if (dtype < VDB_F32 || dtype > VDB_BF16) throw Failure(err_arg("unknown element type"));
@@ -93,14 +97,14 @@ vdb_status vdb_q8_quantize_dev(const void* d_rows, vdb_dtype dtype, size_t strid
         if (__builtin_mul_overflow(stride, size, &bytes)) throw Failure(err_arg("d_rows does not fit the address space"));
         const Range in = range_of(d_rows, out->n, out->dim * size, bytes, "d_rows"), c = codes_of(*out, "out"), s = scales_of(*out, "out"), m = norms_of(*out, "out");
         if (meet(in, c) || meet(in, s) || meet(in, m) || meet(c, s) || meet(c, m) || meet(s, m)) throw Failure(err_arg("the buffers overlap"));
-        OnDevice dev;
+        OnDevice dev(device);
         dev.add(d_rows, "d_rows"); add_rows(dev, *out, out->norms2 != nullptr);
         dev.enter();
         launch_q8_quantize(d_rows, dtype, stride, *out, (hipStream_t)stream);
     });
 }
 
-vdb_status vdb_q8_score_dev(const vdb_q8_rows* queries, const vdb_q8_rows* base, vdb_metric metric, float* d_out, size_t out_stride, void* stream) {
+vdb_status vdb_q8_score_on(int device, const vdb_q8_rows* queries, const vdb_q8_rows* base, vdb_metric metric, float* d_out, size_t out_stride, void* stream) {
     return guard([&] {
         check_rows(queries, "queries"); check_rows(base, "base"); check_metric(metric);
         if (queries->dim != base->dim) throw Failure(err_length_mismatch(base->dim, queries->dim));
@@ -115,11 +119,24 @@ vdb_status vdb_q8_score_dev(const vdb_q8_rows* queries, const vdb_q8_rows* base,
         const Range o = range_of(d_out, queries->n, base->n * 4, bytes, "d_out");
         for (const vdb_q8_rows* r : {queries, base})
             if (meet(o, codes_of(*r, "rows")) || meet(o, scales_of(*r, "rows")) || (norms && meet(o, norms_of(*r, "rows")))) throw Failure(err_arg("d_out overlaps the rows"));
-        OnDevice dev;
+        OnDevice dev(device);
         add_rows(dev, *queries, norms); add_rows(dev, *base, norms); dev.add(d_out, "d_out");
         dev.enter();
         launch_q8_score(view(*queries), view(*base), metric, d_out, out_stride, (hipStream_t)stream);
     });
+}
+
+vdb_status vdb_q8_quantize_dev(const void* d_rows, vdb_dtype dtype, size_t stride, const vdb_q8_rows* out, void* stream) {
+    return vdb_q8_quantize_on(-1, d_rows, dtype, stride, out, stream);
+}
+
+vdb_status vdb_q8_score_dev(const vdb_q8_rows* queries, const vdb_q8_rows* base, vdb_metric metric, float* d_out, size_t out_stride, void* stream) {
+    return vdb_q8_score_on(-1, queries, base, metric, d_out, out_stride, stream);
+}
+
+vdb_status vdb_score_adjust_dev(const float* d_scores, size_t stride, size_t nq, size_t n, vdb_metric metric, const vdb_score_adjust* how,
+                                float* d_out, size_t out_stride, void* stream) {
+    return vdb_score_adjust_on(-1, d_scores, stride, nq, n, metric, how, d_out, out_stride, stream);
 }
 
 vdb_status vdb_q8_score_scan(const float* queries, size_t nq, const float* base, size_t n, size_t dim, vdb_metric metric, int device, float* out) {
@@ -156,8 +173,8 @@ vdb_status vdb_q8_score_scan(const float* queries, size_t nq, const float* base,
     });
 }
 
-vdb_status vdb_score_adjust_dev(const float* d_scores, size_t stride, size_t nq, size_t n, vdb_metric metric, const vdb_score_adjust* how,
-                                float* d_out, size_t out_stride, void* stream) {
+vdb_status vdb_score_adjust_on(int device, const float* d_scores, size_t stride, size_t nq, size_t n, vdb_metric metric, const vdb_score_adjust* how,
+                               float* d_out, size_t out_stride, void* stream) {
     return guard([&] {
         check_metric(metric); need(how, "how");
         if (n > 0xFFFFFFFFull || nq > 0xFFFFFFFFull) throw Failure(err_arg("more than 2^32 - 1 columns or queries"));
@@ -183,7 +200,7 @@ vdb_status vdb_score_adjust_dev(const float* d_scores, size_t stride, size_t nq,
             {a.how.seen, 1, how->n_seen * 4, 0, "seen"}, {a.how.seen_offsets, 1, (nq + 1) * 8, 0, "seen_offsets"},
             {a.how.repeat, 1, nq * 4, 0, "repeat"}, {a.how.frequency, 1, nq * 4, 0, "frequency"}, {a.how.presence, 1, nq * 4, 0, "presence"}};
         for (const auto& b : side) if (b.p && meet(o, range_of(b.p, b.rows, b.row, b.stride, b.what))) throw Failure(err_arg(std::string("d_out overlaps ") + b.what));
-        OnDevice dev;
+        OnDevice dev(device);
         dev.add(d_scores, "d_scores"); dev.add(d_out, "d_out");
         for (const auto& b : side) if (b.p) dev.add(b.p, b.what);
         dev.enter();

@@ -1,6 +1,6 @@
 // vectordb_amd._tensors: the calls of scores.py on torch tensors, as a module of the interpreter.  A call reads addresses, sizes and
-// strides from the tensors that it is given, checks them, allocates its result and calls the C entry point on the current stream of the
-// tensors' device.  In Python the same steps took 4 us of an 8 us call, more than the launch and the kernel of a small one.
+// strides from the tensors that it is given, checks them, allocates its result and calls the entry point on the tensors' device and its current
+// stream.  In Python the same steps took 4 us of an 8 us call, more than the launch and the kernel of a small one.
 // Nothing of a tensor is kept; the interpreter's lock is free while the entry point runs.
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
@@ -10,7 +10,7 @@
 #include <string>
 #include <utility>
 
-#include "../../include/vdbmi.h"
+#include "scores_on.hpp"
 
 namespace {
 
@@ -33,9 +33,9 @@ struct Refusal { std::string why; };                           // becomes an Arg
 template <class T> T* got(T* p) { if (!p) throw Raised{}; return p; }
 
 // What bind() hands over, for the life of the process.
-decltype(&vdb_q8_quantize_dev) quantize_dev;
-decltype(&vdb_q8_score_dev) score_dev;
-decltype(&vdb_score_adjust_dev) adjust_dev;
+decltype(&vdb_q8_quantize_on) quantize_on;
+decltype(&vdb_q8_score_on) score_on;
+decltype(&vdb_score_adjust_on) adjust_on;
 PyObject *rows_class, *check, *argument_error, *length_mismatch, *out_of_memory, *raw_stream, *metrics;
 PyObject *name_codes, *name_scales, *name_norms2, *name_dim, *no_arguments;
 
@@ -256,7 +256,7 @@ PyObject* quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args, PyO
             if (r.c.n != (size_t)x.rows || r.c.dim != (size_t)x.width || r.device != device)
                 refuse("out: expected " + std::to_string(x.rows) + " rows of " + std::to_string(x.width) + " columns on " + text(device));
         }
-        call(device, [&](void* stream) { return quantize_dev(x.p, (vdb_dtype)kind, (size_t)x.stride, &r.c, stream); });
+        call(device, [&](void* stream) { return quantize_on(device.index(), x.p, (vdb_dtype)kind, (size_t)x.stride, &r.c, stream); });
         if (a.v[1] != Py_None)
             for (PyObject* o : {r.codes.p, r.scales.p, r.norms2.p}) if (o != Py_None) written(o);
         return out.take();
@@ -279,7 +279,7 @@ PyObject* score_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args, PyObje
         }
         const int metric = metric_of(a.v[2]);
         Result out = result(a.v[3], (int64_t)q.c.n, (int64_t)b.c.n, b.device);
-        call(b.device, [&](void* stream) { return score_dev(&q.c, &b.c, (vdb_metric)metric, (float*)out.s.p, (size_t)out.s.stride, stream); });
+        call(b.device, [&](void* stream) { return score_on(b.device.index(), &q.c, &b.c, (vdb_metric)metric, (float*)out.s.p, (size_t)out.s.stride, stream); });
         if (a.v[3] != Py_None) written(out.o.p);
         return out.o.take();
     } catch (...) { return set_error(); }
@@ -327,7 +327,7 @@ PyObject* adjust_scores(PyObject*, PyObject* const* args, Py_ssize_t n_args, PyO
         how.frequency = each(FREQUENCY);
         how.presence = each(PRESENCE);
         Result out = result(a.v[OUT], nq, n, device);
-        call(device, [&](void* stream) { return adjust_dev((const float*)s.p, (size_t)s.stride, (size_t)nq, (size_t)n, (vdb_metric)metric, &how, (float*)out.s.p, (size_t)out.s.stride, stream); });
+        call(device, [&](void* stream) { return adjust_on(device.index(), (const float*)s.p, (size_t)s.stride, (size_t)nq, (size_t)n, (vdb_metric)metric, &how, (float*)out.s.p, (size_t)out.s.stride, stream); });
         if (a.v[OUT] != Py_None) written(out.o.p);
         return out.o.take();
     } catch (...) { return set_error(); }
@@ -361,7 +361,7 @@ PyObject* bind(PyObject*, PyObject* args) {
     unsigned long long q, s, a;
     PyObject *rows, *chk, *refused, *mismatch, *oom, *stream, *m;
     if (!PyArg_ParseTuple(args, "KKKOOOOOOO", &q, &s, &a, &rows, &chk, &refused, &mismatch, &oom, &stream, &m)) return nullptr;
-    quantize_dev = (decltype(quantize_dev))(uintptr_t)q; score_dev = (decltype(score_dev))(uintptr_t)s; adjust_dev = (decltype(adjust_dev))(uintptr_t)a;
+    quantize_on = (decltype(quantize_on))(uintptr_t)q; score_on = (decltype(score_on))(uintptr_t)s; adjust_on = (decltype(adjust_on))(uintptr_t)a;
     rows_class = Py_NewRef(rows); check = Py_NewRef(chk); argument_error = Py_NewRef(refused); length_mismatch = Py_NewRef(mismatch); out_of_memory = Py_NewRef(oom); raw_stream = Py_NewRef(stream); metrics = Py_NewRef(m);
     Py_RETURN_NONE;
 }

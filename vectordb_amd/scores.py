@@ -5,7 +5,7 @@
     s = score_rows(q, base, DistanceMetric.Cosine)       # [nq, n] f32
     s = adjust_scores(s, DistanceMetric.Cosine, pass_bits=bits, boost=boost, seen=seen, seen_offsets=offsets, frequency=f)
 
-Each call is one entry point of the C ABI (vdb_q8_quantize_dev, vdb_q8_score_dev, vdb_score_adjust_dev: include/vdbmi.h has
+Each call is one entry point of the library (vdb_q8_quantize_dev, vdb_q8_score_dev, vdb_score_adjust_dev: include/vdbmi.h has
 the formulas and the layout), enqueued on the current stream of the tensors' device; nothing waits.  Tensors must live on one
 GPU; what a call cannot take is refused with ArgumentError before anything is launched, or VectorLengthMismatch for rows of two lengths.
 The calls have no gradient: while gradients are recorded a tensor that requires one is refused, as are tensors with tangents and
@@ -18,7 +18,7 @@ import ctypes as C
 
 import torch
 
-from . import api as _api
+from . import api as _api, load_library
 from .capi import ArgumentError, DistanceMetric, Q8RowsC, VectorLengthMismatch
 
 try:
@@ -65,12 +65,13 @@ class Q8Rows:
 
 
 def _bind():
+    library, a = load_library(), _api()
+
     def address(entry):
-        return C.cast(entry, C.c_void_p).value
-    a = _api()
+        return C.cast(getattr(library, entry), C.c_void_p).value
     # the current stream's handle alone, without a Stream object around it (2 us a call), where torch offers it
     stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
-    bind(address(a.fn.q8_quantize_dev), address(a.fn.q8_score_dev), address(a.fn.score_adjust_dev), Q8Rows, a.check, ArgumentError, VectorLengthMismatch, torch.OutOfMemoryError, stream,
+    bind(address("vdb_q8_quantize_on"), address("vdb_q8_score_on"), address("vdb_score_adjust_on"), Q8Rows, a.check, ArgumentError, VectorLengthMismatch, torch.OutOfMemoryError, stream,
              frozenset(int(m) for m in DistanceMetric))
 
 
