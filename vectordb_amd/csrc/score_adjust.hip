@@ -105,7 +105,9 @@ void launch_score_adjust(const AdjustArgs& a, hipStream_t s) {
     // Every span reads its query's whole list again, so long lists want long spans while they fill the chip (64 x 128000, lists of 3000:
     // 14.4 us, spans of 4096 16.9; of 30000: 29.3 and 60.6); short lists want many workgroups (16 x 1000003, lists of 300: spans of 4096
     // 26.7 us, of 16384 31.8).
-    if (!a.how.seen) launch<4096, 256>(a, s);
+    // Without lists one piece per thread.  With boosts in spans of 4096 / 2048 / 1024 (torch's addition): 145 x 30088 8.1 / 7.8 / 7.3 us (7.6), 256 x 60000
+    // 26.4 / 24.2 / 23.7 (22.2), 16 x 1000003 27.9 / 27.1 / 25.6 (30.2), 4 x 3000000 21.8 / 20.5 / 20.0 (23.2), but 64 x 128000 10.8 / 11.7 / 11.4 (11.8).
+    if (!a.how.seen) launch<1024, 256>(a, s);
     else if (a.how.n_seen / a.nq >= 1024 && ((uint64_t)a.n + 16383) / 16384 * a.nq >= 256) launch<16384, 512>(a, s);
     else launch<4096, 512>(a, s);
 }
