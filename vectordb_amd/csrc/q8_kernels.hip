@@ -345,7 +345,7 @@ __device__ inline float finish(float dot, float nq, float nb, int metric) {
 // holds 32 rows of two queries.  Slot 32 i + r of WM holds row MT r + i (MT = WM / 32), so that MT registers of a lane are consecutive
 // rows: a store writes 128 MT bytes in a row for each of two queries.
 // The scales of four blocks are one word per row, which comes with every step.
-// Bound by power where products prevail (4096 x 32000 x 4096: 875 .. 940 us by card and warmth = 1.14 .. 1.23 PFLOP/s, the matrix pipes busy 63 % of the time at 1.9 GHz; 766 us with
+// Bound by power where products prevail (4096 x 32000 x 4096: 875 .. 940 us by card and warmth = 1.14 .. 1.23 PFLOP/s, the matrix pipes busy 64 % of the time at 1.9 GHz; 766 us with
 // codes that are all equal), by the scores that leave where rows are short (1000 x 1M x 960: 2.07 .. 2.2 ms, 4 GB of them).  On the first of these 16 x 16
 // instructions spill, and two workgroups of 256 x 128 per compute unit are slower; rings of 6, 9 and 12 buffers gain nothing on smaller tiles,
 // nor does letting a tile's stores go on through the next tile's first two steps.
